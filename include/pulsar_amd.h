@@ -34,6 +34,7 @@ extern "C" {
 
 #define PQ_DTYPE_F32 0
 #define PQ_DTYPE_BF16 1
+#define PQ_DTYPE_F16 2
 
 /* Library version string and the calling thread's last error message. */
 const char *pq_version(void);
@@ -508,6 +509,78 @@ int pq_attn_layer_decode(const uint16_t *qkvg, const float *q_norm, const float 
                          const float *rope_cs, uint16_t *kcache, uint16_t *vcache, int pos, int nh,
                          int nkv, int hd, int rot, int win, float eps, float scale, uint16_t *out,
                          int8_t *qx, float *dx, void *stream);
+
+/* ============================================================ paged cache
+ * Many sequences over one pool of cache pages: the cache [ctx][nkv][hd] of
+ * pq_qk_prep / pq_attn_decode cut into pages of `page` positions that may lie
+ * anywhere. No counterpart in the reference (one sequence, one cache).
+ *
+ * Sequence b holds n = kv_len[b] positions, of which the last c are this
+ * call's rows: rows q_start[b] .. q_start[b+1]-1 of its inputs and outputs (c
+ * = their count; q_start ascends), or row b alone where q_start is NULL (then
+ * a call has nseq rows). Row i of the c is position n - c + i. Position j is
+ * slot j % page of page table[b * table_stride + j / page].
+ *
+ * The lengths and the pages are read on the device, so a captured call replays
+ * for other ones. What they hold is checked there, not refused: a page outside
+ * [0, npages), and a position past the row's table_pages, holds no key (nothing is
+ * read or written for it); kv_len <= 0 is a sequence without keys (a padded
+ * batch); rows outside [q_start[0], q_start[nseq]) are left as they were. Pages
+ * may be shared between sequences that only read them. */
+typedef struct pq_paged_kv {
+  uint16_t *k, *v;         /* pools [npages][page][nkv][hd], fp16 or bf16, 16-byte aligned */
+  long long page_stride;   /* elements from page to page of both pools (>= page * nkv * hd, a multiple of 8) */
+  int npages, page;        /* page: a power of two, 8 .. 65536 */
+  int nkv, hd;             /* head_dim 64 or 128 */
+  int dtype;               /* PQ_DTYPE_F16 or PQ_DTYPE_BF16 */
+  const int32_t *table;    /* device [nseq] rows of table_pages page ids, table_stride apart */
+  int table_stride, table_pages;
+  const int32_t *kv_len;   /* device [nseq] */
+  const int32_t *q_start;  /* device [nseq + 1], or NULL: row b is sequence b's one new position */
+  int nseq;
+} pq_paged_kv;
+
+/* The head norm of q and k, RoPE and the cache write (pq_qk_prep) for the T
+ * rows of a batch, in one pass: qkv rows [q (nh hd) | k (nkv hd) | v (nkv hd) |
+ * ...] of row_stride elements, bf16; q_out rows of q_stride elements, bf16
+ * (q_out may be qkv itself with q_stride = row_stride); k and v to the pages.
+ * rope_cs [rope_rows][rot/2][cos, sin] (NULL with rot 0); a row whose position is outside [0,
+ * rope_rows) is left out: its q_out and its slot keep what they held. The
+ * arithmetic is fp32 from the bf16 inputs to one rounding at the end
+ * (pq_qk_prep also rounds after the norm and after its weight, as the
+ * reference's ops do); v is converted (copied for a bf16 pool). Two rows must
+ * not share a slot. */
+int pq_paged_qk_prep(const uint16_t *qkv, int row_stride, uint16_t *q_out, int q_stride, const float *q_norm,
+                     const float *k_norm, const float *rope_cs, int rope_rows, const pq_paged_kv *kv, int nh,
+                     int rot, int T, float eps, void *stream);
+
+/* Attention of one new token a sequence over its pages: row b of q (bf16,
+ * q_stride elements a row) at position p = kv_len[b] - 1 (q_start is not read)
+ * sees the keys j <= p with win == 0, or j > p - win, or j < sinks: a sliding
+ * window whose first `sinks` tokens stay visible. nh / nkv is any whole number
+ * up to 16. s_j = scale * q . k_j, o = sum e^(s_j - max) v_j / sum e^(s_j - max);
+ * out (bf16, out_stride elements a row) = o * sigmoid(gate[b][head]) (gate NULL
+ * for none), rounded once, and/or its Q8_0 form (qx [nseq][nh hd], dx, as
+ * pq_q8_quant_bf16 of out). A row that sees no key gets zeros. What a key
+ * that a row does not see holds (infinities and NaN too) does not reach it.
+ * max_kv: about the largest kv_len (it sets how far the work is split, and
+ * the workspace with it; any length is computed whole). The keys are split over
+ * workgroups and joined in a fixed order: the same call gives the same bits.
+ * ws (16-byte aligned): pq_paged_decode_workspace_bytes, 0 where one workgroup
+ * a kv head does it. */
+size_t pq_paged_decode_workspace_bytes(int nseq, int nh, int nkv, int hd, int max_kv, int win, int sinks);
+int pq_paged_attn_decode(const uint16_t *q, int q_stride, const pq_paged_kv *kv, const uint16_t *gate,
+                         int gate_stride, uint16_t *out, int out_stride, int8_t *qx, float *dx, int nh, float scale,
+                         int win, int sinks, int max_kv, void *ws, size_t ws_bytes, void *stream);
+
+/* The same for prompt rows: T rows of a ragged batch (kv->q_start), each row
+ * at its position p, with the keys of the sequence's earlier rows in the pages
+ * (pq_paged_qk_prep of the batch before it). Rows outside the sequences keep
+ * what they held. */
+size_t pq_paged_prefill_workspace_bytes(int nseq, int T, int nh, int nkv, int hd, int max_kv, int win, int sinks);
+int pq_paged_attn_prefill(const uint16_t *q, int q_stride, const pq_paged_kv *kv, const uint16_t *gate,
+                          int gate_stride, uint16_t *out, int out_stride, int8_t *qx, float *dx, int nh, int T,
+                          float scale, int win, int sinks, int max_kv, void *ws, size_t ws_bytes, void *stream);
 
 /* ======================================================= ternary GEMV
  * PQ2_0 x Q8_K, the Bonsai ternary path. codes u8 [N][K/4] (weight i of a

@@ -1,0 +1,55 @@
+// paged.h -- what the paged-cache kernels share: the device view of a
+// pq_paged_kv, the row -> (sequence, position) map and the visibility rule.
+#pragma once
+#include "pq_device.h"
+#include "pq_host.h"
+
+namespace pq {
+
+// pq_paged_kv as the kernels take it (by value). cap: positions a table row covers.
+struct PagedView {
+  uint16_t *k, *v;
+  long long page_stride;
+  const int32_t *table, *kv_len, *q_start;
+  int npages, lg_page, nkv, nseq, table_stride, cap;
+};
+
+// Checks the struct's host-side fields; fills the view.
+int paged_view(const pq_paged_kv *kv, const char *who, PagedView *out);
+
+// The sequence that row belongs to (the wave's lanes scan q_start together), or
+// -1; first / count: its rows. row must be uniform over the wave.
+__device__ __forceinline__ int paged_seq_of_row(const PagedView &kv, int row, int &first, int &count) {
+  if (kv.q_start == nullptr) {
+    first = row;
+    count = 1;
+    return row < kv.nseq ? row : -1;
+  }
+  const int lane = threadIdx.x & 63;
+  int b = 0;
+  for (int i = 0; i < kv.nseq; i += 64)
+    b += __popcll(__ballot(i + lane < kv.nseq && kv.q_start[i + lane < kv.nseq ? i + lane + 1 : 0] <= row));
+  if (b >= kv.nseq) return -1;
+  first = kv.q_start[b];
+  const int end = kv.q_start[b + 1];
+  count = end - first;
+  return row >= first && row < end ? b : -1;
+}
+
+// Element offset of position j's row of kv heads in the pools, or -1 when it
+// has none (past the table, or a page outside the pool).
+__device__ __forceinline__ long long paged_row(const PagedView &kv, int b, int j, int kvd) {
+  if (j < 0 || j >= kv.cap) return -1;
+  const int id = kv.table[(size_t)b * kv.table_stride + (j >> kv.lg_page)];
+  if (id < 0 || id >= kv.npages) return -1;
+  return id * kv.page_stride + (long long)(j & ((1 << kv.lg_page) - 1)) * kvd;
+}
+
+// fp16 or bf16 cache element -> f32 and back
+template <bool BF>
+__device__ __forceinline__ float kv2f(uint16_t v) {
+  if constexpr (BF) return bf2f(v);
+  else return h2f(v);
+}
+
+}  // namespace pq

@@ -33,6 +33,13 @@ class GemvPrologue(C.Structure):
                 ("tok", C.c_void_p), ("vocab", C.c_int), ("xf", C.c_void_p), ("emb_sf", C.c_void_p)]
 
 
+class PagedKVView(C.Structure):
+    """pq_paged_kv."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_longlong), ("npages", C.c_int),
+                ("page", C.c_int), ("nkv", C.c_int), ("hd", C.c_int), ("dtype", C.c_int), ("table", C.c_void_p),
+                ("table_stride", C.c_int), ("table_pages", C.c_int), ("kv_len", C.c_void_p), ("q_start", C.c_void_p), ("nseq", C.c_int)]
+
+
 SIGNATURES = {
     "pq_version": (C.c_char_p, []),
     "pq_last_error": (C.c_char_p, []),
@@ -92,6 +99,11 @@ SIGNATURES = {
     "pq_q8r_gemv_fused_swiglu": (I, [P, P, C.POINTER(GemvPrologue), P, I, I, P]),
     "pq_q8_gemv_fused_swiglu": (I, [P, P, C.POINTER(GemvPrologue), P, P, I, I, P]),
     "pq_attn_layer_decode": (I, [P, P, P, P, P, P, I, I, I, I, I, I, F, F, P, P, P, P]),
+    "pq_paged_qk_prep": (I, [P, I, P, I, P, P, P, I, C.POINTER(PagedKVView), I, I, I, F, P]),
+    "pq_paged_decode_workspace_bytes": (Z, [I, I, I, I, I, I, I]),
+    "pq_paged_attn_decode": (I, [P, I, C.POINTER(PagedKVView), P, I, P, I, P, P, I, F, I, I, I, P, Z, P]),
+    "pq_paged_prefill_workspace_bytes": (Z, [I, I, I, I, I, I, I, I]),
+    "pq_paged_attn_prefill": (I, [P, I, C.POINTER(PagedKVView), P, I, P, I, P, P, I, I, F, I, I, I, P, Z, P]),
     "pq_tq2_gemv": (I, [P, P, P, P, I, I, P]),
     "pq_tq2_gemv_batch": (I, [P, P, P, P, I, P, I, P]),
     "pq_q8_gemm_scratch_bytes": (Z, []),

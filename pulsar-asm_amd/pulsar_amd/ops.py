@@ -9,13 +9,13 @@ import ctypes as C
 import torch
 
 from . import check, lib
-from ._abi import GemvPrologue
+from ._abi import GemvPrologue, PagedKVView
 
 __all__ = ["stream_ptr", "Q8Weight", "q8_quant", "q8_gemv", "q8_gemm", "q8r_gemv", "q8r_gemv_fused", "QlowWeight", "qlow_gemv", "qlow_gemv_fused", "qlow_gemv_fused_swiglu", "qlow_gemm", "DT_F32", "DT_BF16", "rmsnorm", "qk_prep", "qk_prep_ref", "attn_ref", "attn_decode_ref", "attn_decode_ref_q8gate",
            "attn_decode", "conv", "silu_mul", "argmax", "embed", "q8k_quant", "tq2_gemv", "tq2_gemv_batch", "gemv_fused",
            "gemv_fused_swiglu",
            "argmax_parts", "attn_layer_decode", "q8r_gemv_fused_swiglu", "PRO_Q8", "PRO_RESNORM", "PRO_NORM", "PRO_EMBED", "PRO_SILU",
-           "PRO_CONV", "PRO_F32"]
+           "PRO_CONV", "PRO_F32", "PagedKV", "paged_qk_prep", "paged_attn_decode", "paged_attn_prefill"]
 
 PRO_Q8, PRO_RESNORM, PRO_NORM, PRO_EMBED, PRO_SILU, PRO_CONV, PRO_F32 = 0, 1, 2, 3, 4, 5, 6
 
@@ -453,3 +453,144 @@ def attn_layer_decode(qkvg, q_norm, k_norm, rope_cs, kc, vc, pos, nh, nkv, hd, r
                                      _bits16(out) if out is not None else None, _ptr(qx), _ptr(dx),
                                      stream_ptr()), "pq_attn_layer_decode")
     return qx, dx
+
+
+# --------------------------------------------------------------- paged cache
+_DT_OF = {torch.float16: 2, torch.bfloat16: 1}
+_RAW16 = (torch.bfloat16, torch.int16, torch.uint16)
+
+
+class PagedKV:
+    """A batch's view of a paged cache (pq_paged_kv): the pools k and v
+    [npages][page][nkv][hd] (fp16 or bf16; the page dimension may have any
+    stride that both share), the page table [nseq][pages] and the lengths
+    kv_len [nseq] (int32), and q_start [nseq + 1] (int32) for calls of more than
+    a row a sequence. The tensors are read on the device at each call, so a
+    program fills them anew from step to step and keeps the view."""
+
+    def __init__(self, k, v, table, kv_len, q_start=None):
+        if k.dtype not in _DT_OF or v.dtype != k.dtype or k.dim() != 4 or v.shape != k.shape:
+            raise ValueError("k and v must be fp16 or bf16 pools [npages][page][nkv][hd] of one shape")
+        npages, page, nkv, hd = k.shape
+        for t in (k, v):
+            if t.stride()[1:] != (nkv * hd, hd, 1) or t.stride(0) != k.stride(0):
+                raise ValueError("a pool's pages must be contiguous, and k and v of one page stride")
+        ints = [table, kv_len] + ([q_start] if q_start is not None else [])
+        if any(t.dtype != torch.int32 for t in ints):
+            raise ValueError("table, kv_len and q_start must be int32")
+        if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1 or table.stride(1) != 1 \
+                or table.stride(0) < table.shape[1]:
+            raise ValueError("table must be [nseq][pages] with unit column stride")
+        nseq = table.shape[0]
+        if tuple(kv_len.shape) != (nseq,) or not kv_len.is_contiguous():
+            raise ValueError("kv_len must be a contiguous [nseq] tensor")
+        if q_start is not None and (tuple(q_start.shape) != (nseq + 1,) or not q_start.is_contiguous()):
+            raise ValueError("q_start must be a contiguous [nseq + 1] tensor")
+        if any(t.device != k.device for t in (v, *ints)):
+            raise ValueError("the pools, the table and the lengths must be on one device")
+        self.tensors = (k, v, table, kv_len, q_start)   # kept alive with the view
+        self.npages, self.page, self.nkv, self.hd, self.nseq = npages, page, nkv, hd, nseq
+        self.capacity = table.shape[1] * page
+        self.device = k.device
+        self.index = k.device.index if k.device.type == "cuda" else None
+        c = self.c = PagedKVView()
+        c.k, c.v, c.page_stride = k.data_ptr(), v.data_ptr(), k.stride(0)
+        c.npages, c.page, c.nkv, c.hd, c.dtype = npages, page, nkv, hd, _DT_OF[k.dtype]
+        c.table, c.table_stride, c.table_pages = table.data_ptr(), table.stride(0), table.shape[1]
+        c.kv_len = kv_len.data_ptr()
+        c.q_start, c.nseq = q_start.data_ptr() if q_start is not None else None, nseq
+        self.ref = C.byref(c)
+
+
+def _paged_rows(kv, what, t, width):
+    """Rows [T][>= width] of 16-bit storage on the view's device: (pointer, row stride, T)."""
+    if t.dtype not in _RAW16 or t.dim() != 2 or t.shape[1] < width or t.stride(1) != 1 or t.device != kv.device:
+        raise ValueError(f"{what} must be bf16 rows of at least {width} on the cache's device, unit column stride")
+    return t.data_ptr(), t.stride(0), t.shape[0]
+
+
+def _paged_stream(kv):
+    """The current stream, of the device that the view's tensors are on."""
+    if kv.index is None:
+        raise ValueError("the cache is not on a GPU")
+    s = stream_ptr()
+    if kv.index != torch._C._cuda_getDevice():
+        raise ValueError("the cache is not on the current GPU")
+    return s
+
+
+def paged_qk_prep(kv, qkv, q_norm, k_norm, rope_cs, nh, rot, eps=1e-5, out=None):
+    """Head norm of q and k, RoPE and the cache write for the rows of a batch
+    (pq_paged_qk_prep): qkv rows [q | k | v | ...], rope_cs [positions][rot/2][2]
+    fp32. Returns q [T][nh * hd] (bf16; out may be qkv itself: in place)."""
+    hd, nkv = kv.hd, kv.nkv
+    x, xs, T = _paged_rows(kv, "qkv", qkv, (nh + 2 * nkv) * hd)
+    if any(t.dtype != torch.float32 or not t.is_contiguous() or t.device != kv.device for t in (q_norm, k_norm, rope_cs)):
+        raise ValueError("the norm weights and the RoPE table must be contiguous fp32 on the cache's device")
+    if q_norm.numel() != hd or k_norm.numel() != hd or tuple(rope_cs.shape[1:]) != (rot // 2, 2):
+        raise ValueError("the norm weights must hold head_dim values, the RoPE table [positions][rot/2][2]")
+    if out is None:
+        out = torch.empty((T, nh * hd), dtype=torch.bfloat16, device=qkv.device)
+    y, ys, Ty = _paged_rows(kv, "out", out, nh * hd)
+    if Ty != T:
+        raise ValueError("out must have a row for each of qkv's")
+    check(lib().pq_paged_qk_prep(x, xs, y, ys, q_norm.data_ptr(), k_norm.data_ptr(), rope_cs.data_ptr(),
+                                 rope_cs.shape[0], kv.ref, nh, rot, T, eps, _paged_stream(kv)), "pq_paged_qk_prep")
+    return out
+
+
+def _paged_attn(kv, q, nh, scale, gate, win, sinks, max_kv, out, qx, dx, ws, prefill):
+    n = nh * kv.hd
+    qp, qs, T = _paged_rows(kv, "q", q, n)
+    if not prefill and T != kv.nseq:
+        raise ValueError("q must have a row for each sequence")
+    gp, gs = None, 0
+    if gate is not None:
+        gp, gs, Tg = _paged_rows(kv, "gate", gate, nh)
+        if Tg != T:
+            raise ValueError("gate must have a row for each of q's")
+    if out is None and qx is None:
+        out = torch.empty((T, n), dtype=torch.bfloat16, device=q.device)
+    op, os = None, 0
+    if out is not None:
+        op, os, To = _paged_rows(kv, "out", out, n)
+        if To != T:
+            raise ValueError("out must have a row for each of q's")
+    if qx is not None and (dx is None or qx.dtype != torch.int8 or dx.dtype != torch.float32 or tuple(qx.shape) != (T, n)
+                           or tuple(dx.shape) != (T, n // 32) or not qx.is_contiguous() or not dx.is_contiguous()
+                           or qx.device != kv.device or dx.device != kv.device):
+        raise ValueError("qx must be int8 [T][nh * hd], dx fp32 [T][nh * hd / 32], contiguous on the cache's device")
+    if max_kv is None:
+        max_kv = kv.capacity
+    L = lib()
+    if prefill:
+        need = L.pq_paged_prefill_workspace_bytes(kv.nseq, T, nh, kv.nkv, kv.hd, max_kv, win, sinks)
+    else:
+        need = L.pq_paged_decode_workspace_bytes(kv.nseq, nh, kv.nkv, kv.hd, max_kv, win, sinks)
+    if need and ws is None:
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    wp, wn = (ws.data_ptr(), ws.numel() * ws.element_size()) if ws is not None else (None, 0)
+    st = _paged_stream(kv)
+    if prefill:
+        check(L.pq_paged_attn_prefill(qp, qs, kv.ref, gp, gs, op, os, _ptr(qx), _ptr(dx), nh, T, scale, win, sinks, max_kv,
+                                      wp, wn, st), "pq_paged_attn_prefill")
+    else:
+        check(L.pq_paged_attn_decode(qp, qs, kv.ref, gp, gs, op, os, _ptr(qx), _ptr(dx), nh, scale, win, sinks, max_kv,
+                                     wp, wn, st), "pq_paged_attn_decode")
+    return out
+
+
+def paged_attn_decode(kv, q, nh, scale, gate=None, win=0, sinks=0, max_kv=None, out=None, qx=None, dx=None, ws=None):
+    """Attention of one new token a sequence over its pages
+    (pq_paged_attn_decode): q rows [nseq][nh * hd ...] bf16, gate rows [nseq][nh].
+    win > 0: a sliding window whose first `sinks` tokens stay visible. max_kv:
+    about the largest length (the table's capacity if not given). Returns out
+    (bf16 [nseq][nh * hd]); qx / dx receive its Q8_0 form."""
+    return _paged_attn(kv, q, nh, scale, gate, win, sinks, max_kv, out, qx, dx, ws, False)
+
+
+def paged_attn_prefill(kv, q, nh, scale, gate=None, win=0, sinks=0, max_kv=None, out=None, qx=None, dx=None, ws=None):
+    """paged_attn_decode for the rows of a ragged batch (pq_paged_attn_prefill):
+    q [T][nh * hd ...], rows q_start[b] .. q_start[b + 1] - 1 the last positions
+    of sequence b. Rows of no sequence keep what out held."""
+    return _paged_attn(kv, q, nh, scale, gate, win, sinks, max_kv, out, qx, dx, ws, True)
