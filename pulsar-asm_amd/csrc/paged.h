@@ -16,6 +16,10 @@ struct PagedView {
 
 // Checks the struct's host-side fields; fills the view.
 int paged_view(const pq_paged_kv *kv, const char *who, PagedView *out);
+// The checks that both attentions share, the view's among them.
+int paged_attn_check(const char *who, const uint16_t *q, int q_stride, const pq_paged_kv *kv, const uint16_t *gate,
+                     int gate_stride, const uint16_t *out, int out_stride, const int8_t *qx, const float *dx, int nh,
+                     int win, int sinks, int max_kv, PagedView *v);
 
 // The sequence that row belongs to (the wave's lanes scan q_start together), or
 // -1; first / count: its rows. row must be uniform over the wave.

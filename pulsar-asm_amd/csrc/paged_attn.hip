@@ -100,19 +100,14 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(const uint16_t *__restr
 
 using namespace pq;
 
-static int paged_attn(const char *who, const uint16_t *q, int q_stride, const pq_paged_kv *kv, bool one_each,
-                      const uint16_t *gate, int gate_stride, uint16_t *out, int out_stride, int8_t *qx, float *dx,
-                      int nh, int T, float scale, int win, int sinks, int max_kv, void *stream) {
-  PQ_REQUIRE(q && (out || qx) && (!qx || dx), PQ_ERR_ARG, "%s: null pointer", who);
+static int paged_attn(const char *who, const uint16_t *q, int q_stride, const pq_paged_kv *kv, const uint16_t *gate,
+                      int gate_stride, uint16_t *out, int out_stride, int8_t *qx, float *dx, int nh, int T, float scale,
+                      int win, int sinks, int max_kv, void *stream) {
   PagedView v;
-  const int rc = paged_view(kv, who, &v);
+  const int rc = paged_attn_check(who, q, q_stride, kv, gate, gate_stride, out, out_stride, qx, dx, nh, win, sinks, max_kv, &v);
   if (rc) return rc;
-  PQ_REQUIRE(nh > 0 && nh % v.nkv == 0 && nh / v.nkv <= 16 && T > 0 && win >= 0 && sinks >= 0 && max_kv > 0, PQ_ERR_ARG,
-             "%s: nh=%d nkv=%d T=%d win=%d sinks=%d max_kv=%d", who, nh, v.nkv, T, win, sinks, max_kv);
-  PQ_REQUIRE(q_stride >= nh * kv->hd && (!out || out_stride >= nh * kv->hd) && (!gate || gate_stride >= nh), PQ_ERR_ARG,
-             "%s: row strides %d, %d and %d too small", who, q_stride, out_stride, gate_stride);
-  if (one_each) v.q_start = nullptr;
-  PQ_REQUIRE(v.q_start || T == kv->nseq, PQ_ERR_ARG, "%s: %d rows for %d sequences without q_start", who, T, kv->nseq);
+  PQ_REQUIRE(T > 0 && (v.q_start || T == kv->nseq), PQ_ERR_ARG, "%s: %d rows for %d sequences%s", who, T, kv->nseq,
+             v.q_start ? "" : " without q_start");
 #define PQ_ATT(HH, BB)                                                                                               \
   launch(paged_attn_kernel<HH, BB>, dim3(T, nh), dim3(256), 0, as_stream(stream), q, q_stride, v, gate, gate_stride, \
          out, out_stride, qx, dx, nh, scale, win, sinks)
@@ -128,18 +123,6 @@ static int paged_attn(const char *who, const uint16_t *q, int q_stride, const pq
   return check_launch(who);
 }
 
-extern "C" size_t pq_paged_decode_workspace_bytes(int nseq, int nh, int nkv, int hd, int max_kv, int win, int sinks) {
-  return 0;
-}
-
-extern "C" int pq_paged_attn_decode(const uint16_t *q, int q_stride, const pq_paged_kv *kv, const uint16_t *gate,
-                                    int gate_stride, uint16_t *out, int out_stride, int8_t *qx, float *dx, int nh,
-                                    float scale, int win, int sinks, int max_kv, void *ws, size_t ws_bytes,
-                                    void *stream) {
-  return paged_attn("pq_paged_attn_decode", q, q_stride, kv, true, gate, gate_stride, out, out_stride, qx, dx, nh,
-                    kv ? kv->nseq : 0, scale, win, sinks, max_kv, stream);
-}
-
 extern "C" size_t pq_paged_prefill_workspace_bytes(int nseq, int T, int nh, int nkv, int hd, int max_kv, int win,
                                                    int sinks) {
   return 0;
@@ -149,6 +132,6 @@ extern "C" int pq_paged_attn_prefill(const uint16_t *q, int q_stride, const pq_p
                                      int gate_stride, uint16_t *out, int out_stride, int8_t *qx, float *dx, int nh,
                                      int T, float scale, int win, int sinks, int max_kv, void *ws, size_t ws_bytes,
                                      void *stream) {
-  return paged_attn("pq_paged_attn_prefill", q, q_stride, kv, false, gate, gate_stride, out, out_stride, qx, dx, nh, T,
+  return paged_attn("pq_paged_attn_prefill", q, q_stride, kv, gate, gate_stride, out, out_stride, qx, dx, nh, T,
                     scale, win, sinks, max_kv, stream);
 }

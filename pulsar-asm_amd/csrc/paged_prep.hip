@@ -12,7 +12,8 @@ int paged_view(const pq_paged_kv *kv, const char *who, PagedView *out) {
              who, kv->dtype);
   PQ_REQUIRE(kv->page >= 8 && kv->page <= 65536 && (kv->page & (kv->page - 1)) == 0, PQ_ERR_ARG,
              "%s: page of %d positions (a power of two, 8 .. 65536)", who, kv->page);
-  PQ_REQUIRE(kv->nkv > 0 && kv->nkv <= 1024 && kv->npages > 0 && kv->table_pages > 0 && kv->table_stride >= kv->table_pages && kv->nseq > 0, PQ_ERR_ARG,
+  PQ_REQUIRE(kv->nkv > 0 && kv->nkv <= 1024 && kv->npages > 0 && kv->table_pages > 0 && kv->table_stride >= kv->table_pages &&
+                 kv->nseq > 0 && kv->nseq <= 65535, PQ_ERR_ARG,
              "%s: nkv=%d npages=%d table %d pages of %d, nseq=%d", who, kv->nkv, kv->npages, kv->table_pages, kv->table_stride,
              kv->nseq);
   PQ_REQUIRE(kv->page_stride >= (long long)kv->page * kv->nkv * kv->hd && kv->page_stride % 8 == 0, PQ_ERR_ARG,
@@ -30,7 +31,20 @@ int paged_view(const pq_paged_kv *kv, const char *who, PagedView *out) {
   out->nseq = kv->nseq;
   out->table_stride = kv->table_stride;
   const long long cap = (long long)kv->table_pages * kv->page;
-  out->cap = cap < 0x7fffffffLL ? (int)cap : 0x7fffffff;
+  out->cap = cap < 0x7fffff00LL ? (int)cap : 0x7fffff00;   // room for a tile's end in an int
+  return PQ_OK;
+}
+
+int paged_attn_check(const char *who, const uint16_t *q, int q_stride, const pq_paged_kv *kv, const uint16_t *gate,
+                     int gate_stride, const uint16_t *out, int out_stride, const int8_t *qx, const float *dx, int nh,
+                     int win, int sinks, int max_kv, PagedView *v) {
+  PQ_REQUIRE(q && (out || qx) && (!qx || dx), PQ_ERR_ARG, "%s: null pointer", who);
+  const int rc = paged_view(kv, who, v);
+  if (rc) return rc;
+  PQ_REQUIRE(nh > 0 && nh % v->nkv == 0 && nh / v->nkv <= 16 && win >= 0 && sinks >= 0 && max_kv > 0, PQ_ERR_ARG,
+             "%s: nh=%d nkv=%d win=%d sinks=%d max_kv=%d", who, nh, v->nkv, win, sinks, max_kv);
+  PQ_REQUIRE(q_stride >= nh * kv->hd && (!out || out_stride >= nh * kv->hd) && (!gate || gate_stride >= nh), PQ_ERR_ARG,
+             "%s: row strides %d, %d and %d too small", who, q_stride, out_stride, gate_stride);
   return PQ_OK;
 }
 

@@ -39,7 +39,7 @@ def _prefill(view, q=64, qs=3104, gate=64, gs=3104, out=64, os=2048, qx=None, dx
     (dict(k=None), ARG, b"null"), (dict(v=None), ARG, b"null"), (dict(table=None), ARG, b"null"),
     (dict(kv_len=None), ARG, b"null"), (dict(hd=96), ARG, b"head_dim"), (dict(dtype=0), ARG, b"type"),
     (dict(page=4), ARG, b"page"), (dict(page=48), ARG, b"page"), (dict(page=131072), ARG, b"page"),
-    (dict(npages=0), ARG, b"npages"), (dict(nkv=0), ARG, b"nkv"), (dict(nseq=0), ARG, b"nseq"),
+    (dict(npages=0), ARG, b"npages"), (dict(nkv=0), ARG, b"nkv"), (dict(nseq=0), ARG, b"nseq"), (dict(nseq=65536), ARG, b"nseq"),
     (dict(table_pages=0), ARG, b"table"), (dict(table_stride=3), ARG, b"table"),
     (dict(page_stride=16 * 8 * 64 - 8), ARG, b"stride"), (dict(page_stride=16 * 8 * 64 + 4), ARG, b"stride"),
     (dict(k=4104), ALIGN, b"aligned"), (dict(v=8200), ALIGN, b"aligned")])
