@@ -537,7 +537,7 @@ typedef struct pq_paged_kv {
   int table_stride, table_pages;
   const int32_t *kv_len;   /* device [nseq] */
   const int32_t *q_start;  /* device [nseq + 1], or NULL: row b is sequence b's one new position */
-  int nseq;                /* at most 65535 */
+  int nseq;                /* at most 65535, and 2^23 with nkv; a call has at most 2^23 rows */
 } pq_paged_kv;
 
 /* The head norm of q and k, RoPE and the cache write (pq_qk_prep) for the T

@@ -106,7 +106,7 @@ static int paged_attn(const char *who, const uint16_t *q, int q_stride, const pq
   PagedView v;
   const int rc = paged_attn_check(who, q, q_stride, kv, gate, gate_stride, out, out_stride, qx, dx, nh, win, sinks, max_kv, &v);
   if (rc) return rc;
-  PQ_REQUIRE(T > 0 && (v.q_start || T == kv->nseq), PQ_ERR_ARG, "%s: %d rows for %d sequences%s", who, T, kv->nseq,
+  PQ_REQUIRE(T > 0 && T <= 1 << 23 && (v.q_start || T == kv->nseq), PQ_ERR_ARG, "%s: %d rows for %d sequences%s", who, T, kv->nseq,
              v.q_start ? "" : " without q_start");
 #define PQ_ATT(HH, BB)                                                                                               \
   launch(paged_attn_kernel<HH, BB>, dim3(T, nh), dim3(256), 0, as_stream(stream), q, q_stride, v, gate, gate_stride, \

@@ -41,6 +41,7 @@ int paged_attn_check(const char *who, const uint16_t *q, int q_stride, const pq_
   PQ_REQUIRE(q && (out || qx) && (!qx || dx), PQ_ERR_ARG, "%s: null pointer", who);
   const int rc = paged_view(kv, who, v);
   if (rc) return rc;
+  PQ_REQUIRE((long long)v->nseq * v->nkv <= 1 << 23, PQ_ERR_ARG, "%s: nseq=%d x nkv=%d (at most 2^23)", who, v->nseq, v->nkv);
   PQ_REQUIRE(nh > 0 && nh % v->nkv == 0 && nh / v->nkv <= 16 && win >= 0 && sinks >= 0 && max_kv > 0, PQ_ERR_ARG,
              "%s: nh=%d nkv=%d win=%d sinks=%d max_kv=%d", who, nh, v->nkv, win, sinks, max_kv);
   PQ_REQUIRE(q_stride >= nh * kv->hd && (!out || out_stride >= nh * kv->hd) && (!gate || gate_stride >= nh), PQ_ERR_ARG,
@@ -111,7 +112,8 @@ extern "C" int pq_paged_qk_prep(const uint16_t *qkv, int row_stride, uint16_t *q
   PagedView v;
   const int rc = paged_view(kv, "pq_paged_qk_prep", &v);
   if (rc) return rc;
-  PQ_REQUIRE(nh > 0 && nh <= 16 * v.nkv && nh % v.nkv == 0 && rot >= 0 && rot <= kv->hd && rot % 2 == 0 && T > 0 && rope_rows > 0,
+  PQ_REQUIRE(nh > 0 && nh <= 16 * v.nkv && nh % v.nkv == 0 && rot >= 0 && rot <= kv->hd && rot % 2 == 0 && T > 0 && T <= 1 << 23 &&
+                 rope_rows > 0,
              PQ_ERR_ARG, "pq_paged_qk_prep: nh=%d nkv=%d rot=%d T=%d rope_rows=%d", nh, v.nkv, rot, T, rope_rows);
   PQ_REQUIRE(row_stride >= (nh + 2 * v.nkv) * kv->hd && q_stride >= nh * kv->hd, PQ_ERR_ARG,
              "pq_paged_qk_prep: row strides %d and %d too small", row_stride, q_stride);

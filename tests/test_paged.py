@@ -74,7 +74,9 @@ def test_rows_without_q_start():
 def test_bad_attention(bad):
     for call in (_decode, _prefill):
         assert call(_view(), **bad) == ARG, (call.__name__, bad)
-    assert _prefill(_view(), T=0) == ARG
+    for T in (0, (1 << 23) + 1):
+        assert _prefill(_view(), T=T) == ARG and _prep(_view(), T=T) == ARG
+    assert _decode(_view(nkv=1024, nseq=65535, page_stride=1 << 20), nh=1024, qs=65536, os=65536, gs=1024) == ARG
 
 
 def _tensors(nseq=2, pages=3, dtype=torch.float16):
