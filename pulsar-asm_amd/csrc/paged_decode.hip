@@ -69,45 +69,6 @@ __device__ __forceinline__ v4f mfma16(v4u a, v4u b, v4f c) {
 
 __device__ __forceinline__ uint32_t f2h2(float a, float b) { return (uint32_t)f2h(a) | (uint32_t)f2h(b) << 16; }
 
-// Four adjacent dims (d0 a multiple of 4) of one row's head, o unnormalized with
-// the sum l: the division, the gate, the one rounding to bf16, and the Q8_0 form
-// (a block is 8 adjacent threads' dims). some: the row sees a key.
-template <int HD>
-__device__ __forceinline__ void paged_store4(const float *o, float l, bool some, int row, int h, int d0, int nh,
-                                             const uint16_t *gate, int gate_stride, uint16_t *out, int out_stride,
-                                             int8_t *qx, float *dx) {
-  float f = 1.0f / l;
-  if (gate != nullptr) f = f / (1.0f + expf_pq(-bf2f(gate[(size_t)row * gate_stride + h])));
-  uint16_t r[4];
-#pragma unroll
-  for (int i = 0; i < 4; i++) r[i] = some ? f2bf(o[i] * f) : 0;
-  if (out != nullptr) {
-    uint16_t *dst = out + (size_t)row * out_stride + h * HD + d0;
-    if (((uintptr_t)dst & 7) == 0) {
-      *reinterpret_cast<uint2 *>(dst) = make_uint2(r[0] | (uint32_t)r[1] << 16, r[2] | (uint32_t)r[3] << 16);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; i++) dst[i] = r[i];
-    }
-  }
-  if (qx != nullptr) {
-    float a = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; i++) a = fmaxf(a, fabsf(bf2f(r[i])));
-    a = fmaxf(a, dpp_f<kDppXor1>(a));
-    a = fmaxf(a, dpp_f<kDppXor2>(a));
-    a = fmaxf(a, dpp_f<kDppHalfMirror>(a));
-    const float d = a / 127.0f;
-    const Q8Div dv(d);
-    const size_t at = ((size_t)row * nh + h) * HD + d0;
-    uint32_t q = 0;
-#pragma unroll
-    for (int i = 0; i < 4; i++) q |= (uint32_t)(uint8_t)(int8_t)q8_code(dv.div(bf2f(r[i]))) << (8 * i);
-    __builtin_memcpy(qx + at, &q, 4);
-    if ((d0 & 31) == 0) dx[at / 32] = d;
-  }
-}
-
 // A workgroup's 4 waves are HW kv heads (a group) by KW = 4 / HW ways through the
 // keys. A segment is a group of one sequence, its work the sequence's tiles.
 //
