@@ -40,6 +40,12 @@ __device__ __forceinline__ int paged_seq_of_row(const PagedView &kv, int row, in
   return row >= first && row < end ? b : -1;
 }
 
+// kv_len[b], a length below any call's rows standing for none (so that a row's position does not wrap)
+__device__ __forceinline__ int paged_len(const PagedView &kv, int b) {
+  const int n = kv.kv_len[b];
+  return n < -(1 << 24) ? -(1 << 24) : n;
+}
+
 // Element offset of position j's row of kv heads in the pools, or -1 when it
 // has none (past the table, or a page outside the pool).
 __device__ __forceinline__ long long paged_row(const PagedView &kv, int b, int j, int kvd) {

@@ -114,9 +114,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_prefill_kernel(PrefillArgs A
   const int rows = (q1 - q0) * G, r0 = (slot - ((int)((long long)q0 * G / BM) + b)) * BM;
   if (r0 >= rows) return;
   // positions: row i of the sequence is at p0 + i
-  int n = kv.kv_len[b];
-  if (n < -(1 << 24)) n = -(1 << 24);
-  const int p0 = n - (q1 - q0);
+  const int p0 = paged_len(kv, b) - (q1 - q0);
   const int rlast = r0 + BM < rows ? r0 + BM - 1 : rows - 1;
   const int pmin = p0 + r0 / G, pmax = p0 + rlast / G;
   const int limit = pmax + 1 < kv.cap ? pmax + 1 : kv.cap;                 // keys from here on are no row's
@@ -128,7 +126,8 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_prefill_kernel(PrefillArgs A
   const int nt = st + (te > wt ? te - wt : 0);
   const int each = (nt + A.nsplit - 1) / A.nsplit;
   const int t0 = blockIdx.y * each, t1 = t0 + each < nt ? t0 + each : nt;
-  auto tile_base = [&](int i) { return (i < st ? i : i - st + wt) * kKeys; };
+  const int gap = wt - st;
+  auto tile_base = [&](int i) { return (i < st ? i : i + gap) * kKeys; };
   // this lane's row
   const int r = r0 + 32 * w + m, rc = r < rows ? r : rows - 1;
   const int qi = rc / G, head = g * G + (rc - qi * G), row = q0 + qi, pos = p0 + qi;
@@ -153,11 +152,14 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_prefill_kernel(PrefillArgs A
   // Written as asm so that its completion is waited for where the tile is taken up and not at every read of LDS.
   const uint32_t lds0 = (uint32_t)(size_t)(lds_char *)smem;
   auto dma = [&](const char *src, uint32_t off, uint32_t dst) {   // src uniform
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds0 + dst), "v"(off), "s"(src) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds0 + dst), "v"(off), "s"(src) : "memory");
   };
   auto dma_each = [&](const char *src, uint32_t dst) {            // src each lane's own
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds0 + dst), "v"(src) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds0 + dst), "v"(src) : "memory");
   };
+  const char *const kbase = reinterpret_cast<const char *>(kv.k + g * HD), *const vbase = reinterpret_cast<const char *>(kv.v + g * HD);
+  const long long pstride = kv.page_stride * 2;
+  const int kvd2 = kvd * 2;
   auto load = [&](int i, int buf, int ids) {
     const int base = tile_base(i);
 #pragma unroll
@@ -165,8 +167,8 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_prefill_kernel(PrefillArgs A
       const int piece = w + x * NW, r0p = base + piece * RPI;
       const int id = __builtin_amdgcn_readlane(ids, piece * RPI / 8);
       const bool page = (unsigned)id < (unsigned)kv.npages;
-      const long long at = (page ? id : 0) * kv.page_stride + (long long)(r0p & smask) * kvd + g * HD;
-      const char *ks = reinterpret_cast<const char *>(kv.k + at), *vs = reinterpret_cast<const char *>(kv.v + at);
+      const long long at = (page ? id : 0) * pstride + (long long)(r0p & smask) * kvd2;
+      const char *ks = kbase + at, *vs = vbase + at;
       const uint32_t dst = buf * 2 * TB + piece * 1024;
       if (page && r0p + RPI <= limit) {
         dma(ks, offk, dst);
@@ -186,6 +188,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_prefill_kernel(PrefillArgs A
   // scaled by the power of two that brings the row's largest value into [1, 2): exact but for what lies 2^-25 below it
   v4u qf[S];
   float sc = fabsf(A.scale) * 1.44269504088896341f;
+  if (sc == 0.0f) sc = 0x1p-126f;   // a scale of 0: weights of 1, and a hidden score's product still -infinity
   {
     const uint16_t *qr = A.q + (size_t)row * A.q_stride + (size_t)head * HD + 8 * h;
     const uint32_t flip = A.scale < 0.0f ? 0x80008000u : 0u;
@@ -269,20 +272,16 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_prefill_kernel(PrefillArgs A
     mt = max3(mt, s[1][15], mt);
     return max_half_pair(mt) * sc;
   };
-  // the weights and their sum; vis: the scores that are seen (a bit each)
-  auto weights = [&](const v16f(&s)[2], v4u(&p)[4], auto ALL, uint32_t vis) {
+  // the weights and their sum
+  auto weights = [&](const v16f(&s)[2], v4u(&p)[4]) {
     const float off = (mx == -__builtin_inff() ? 0.0f : mx) - kLift;
     float ls[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int u = 0; u < 2; u++)
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
-        float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], sc, -off));
-        float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i + 1], sc, -off));
-        if constexpr (!ALL.value) {
-          x0 = vis & 1u << (16 * u + i) ? x0 : 0.0f;
-          x1 = vis & 1u << (16 * u + i + 1) ? x1 : 0.0f;
-        }
+        const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], sc, -off));
+        const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i + 1], sc, -off));
         ls[(i >> 1) & 3] += x0 + x1;
         p[2 * u + (i >> 3)][(i & 7) >> 1] = pack2<BF>(x0, x1);
       }
@@ -292,19 +291,22 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_prefill_kernel(PrefillArgs A
   auto edge_tile = [&](int buf, int base, uint32_t pages, bool whole) {
     v16f s[2];
     scores(s, buf);
-    // key of score i of half u: base + 32 u + 16 (i / 8) + 8 h + i % 8
-    auto sees = [&](int key, int group) {
-      return key <= pos && key < limit && (key > low || key < A.sinks) && (pages >> group & 1u);
-    };
+    // The lane's scores are four runs of 8 adjacent keys, run r at base + 16 r + 8 h (one page group each): what is seen
+    // of a run is cut out of its 8 bits by the row's bounds. A score that is not seen becomes -infinity, its weight 0.
+    auto first = [](int k) { return (1u << (k < 0 ? 0 : k > 8 ? 8 : k)) - 1u; };   // the run's first k keys
     uint32_t vis = 0;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const int at = base + 16 * r + 8 * h, end = pos < limit ? pos + 1 : limit;
+      const uint32_t run = first(end - at) & (~first(low + 1 - at) | first(A.sinks - at));
+      vis |= (pages >> (2 * r + h) & 1u ? run & 0xffu : 0u) << (8 * r);
+    }
 #pragma unroll
     for (int u = 0; u < 2; u++)
 #pragma unroll
       for (int i = 0; i < 16; i++) {
-        const int off = 32 * u + 16 * (i >> 3) + 8 * h;
-        const bool see = sees(base + off + (i & 7), off >> 3);
-        vis |= see ? 1u << (16 * u + i) : 0u;
-        s[u][i] = see ? s[u][i] : -__builtin_inff();
+        const uint32_t see = (uint32_t)((int)(vis << (31 - 16 * u - i)) >> 31);   // all ones, or none
+        s[u][i] = __uint_as_float((__float_as_uint(s[u][i]) & see) | (0xff800000u & ~see));
       }
     if (!__any(vis != 0)) return;
     some = some || vis != 0;
@@ -320,7 +322,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_prefill_kernel(PrefillArgs A
       mx = mn;
     }
     v4u p[4];
-    weights(s, p, std::false_type{}, vis);
+    weights(s, p);
     if (!whole && __any(lane < NW ? odd_flag[buf][lane < NW ? lane : 0] != 0 : false)) {
       // finite values through the products, the others to the rows that see them: they stay what they are under
       // any weight
@@ -334,7 +336,8 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_prefill_kernel(PrefillArgs A
           o[i] = mfma32<BF>(f, p[k], o[i]);
         }
       for (int key = 0; key < kKeys; key++) {
-        const bool see = sees(base + key, key >> 3);
+        const int j = base + key;
+        const bool see = j <= pos && j < limit && (j > low || j < A.sinks) && (pages >> (key >> 3) & 1u);
         const int sw = HD == 128 ? 4 * (key & 3) : 4 * ((key >> 1) & 1);
 #pragma unroll
         for (int i = 0; i < N; i++)
@@ -355,10 +358,10 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_prefill_kernel(PrefillArgs A
 #pragma unroll
       for (int i = 0; i < N; i++) o[i] = mfma32<BF>(v_frag(buf, i, k), p[k], o[i]);
   };
-  // a tile that every row of the workgroup sees whole; pages: the 8-key groups whose page exists
-  auto inner = [&](int base) {
-    return base + kKeys <= pmin + 1 && base + kKeys <= kv.cap && (A.win == 0 || base > pmax - A.win || base + kKeys <= A.sinks);
-  };
+  // the tiles [ta, te_) of the window that every row of the workgroup sees whole, if their pages exist
+  const int from = A.win > 0 && pmax >= A.win ? (pmax - A.win) / kKeys + 1 : 0, upto = (pmin + 1 < kv.cap ? pmin + 1 : kv.cap) / kKeys;
+  const int ta = from > wt ? from - gap : st, te_ = upto - gap < t1 ? upto - gap : t1;
+  // the 8-key groups of a tile whose page exists
   auto pages_of = [&](int x) { return (uint32_t)__ballot((unsigned)x < (unsigned)kv.npages) & 0xffu; };
   // every wave has its pieces of tile t and has left tile t - 1: t + 1 may be loaded into that one's buffer
   auto take_up = [&](int t, int buf) {
@@ -392,7 +395,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_prefill_kernel(PrefillArgs A
     taken = false;
     t++;
     // the run of inner tiles, most of a long prompt's: a wave leaves it where its sums have to be rescaled
-    while (t < t1 && inner(tile_base(t)) && pages_of(ids) == 0xffu) {
+    while (t >= ta && t < te_ && pages_of(ids) == 0xffu) {
       const int buf = (t - t0) & 1;
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       take_up(t, buf);
@@ -405,7 +408,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_prefill_kernel(PrefillArgs A
       }
       some = true;
       v4u p[4];
-      weights(s, p, std::true_type{}, 0);
+      weights(s, p);
 #pragma unroll
       for (int k = 0; k < 4; k++)
 #pragma unroll
@@ -502,18 +505,20 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillArgs A, 
 }
 
 // The row tile's waves and the splits of the keys: tiles of 256 rows where they
-// fill the chip (head_dim 128: K and V are then read half as often), else of 128; and
-// splits until one workgroup of 256 rows, or two of 128, a CU have work, each of at
-// least 2 tiles of keys. Measured, 256 / 128 rows (us): 16384 queries of 16 q and 4 kv heads
-// of 128 1132 / 1180; 512 behind 32000 in 8 splits 208 / 228; 203 behind 300 unsplit 38 /
-// 38, in 4 splits of 128 rows 25.
+// fill the chip and see 1024 keys or more (head_dim 128: K and V are then read half as often), else
+// of 128; and splits until one workgroup of 256 rows, or two of 128, a CU have
+// work, each of at least 2 tiles of keys. Measured, 256 / 128 rows (us): 16384 queries of 16 q
+// and 4 kv heads of 128 1082 / 1124, 16 sequences of 4096 1293 / 1353, 32 of 2048 786 / 801,
+// 16384 in a window of 256 127 / 107; head_dim 64, 32 and 8 heads, 8192 queries 448 / 424;
+// 203 queries behind 300 unsplit 26 / 22, in 3 splits of 128 rows 18.6; 512 behind 32000
+// unsplit 838 / 699, in 8 splits of 128 rows 158.
 struct PrefillPlan {
   int nw, slots, nsplit;
 };
 static PrefillPlan prefill_plan(int nseq, int T, int nh, int nkv, int hd, int max_kv, int win, int sinks) {
   PrefillPlan p;
   const long long rows = (long long)T * (nh / nkv);
-  p.nw = hd == 128 && (rows + 255) / 256 * nkv >= 256 ? 8 : 4;
+  p.nw = hd == 128 && (rows + 255) / 256 * nkv >= 256 && (win == 0 || win + (long long)sinks >= 1024) && max_kv >= 1024 ? 8 : 4;
   const int BM = 32 * p.nw;
   p.slots = (int)(rows / BM) + nseq;
   const long long groups = (rows + BM - 1) / BM * nkv, fill = 256 * (8 / p.nw) / groups;
