@@ -49,56 +49,125 @@ int paged_attn_check(const char *who, const uint16_t *q, int q_stride, const pq_
   return PQ_OK;
 }
 
-// One wave per (head, row); lane l holds dimensions l + 64e.
+// A wave takes one row and groups of 8 heads of it: lane (u, c) = (lane / TH, lane %
+// TH), TH = HD / 16 lanes a head, holds dims 8 c .. + 7 and HD / 2 + 8 c .. + 7 of head u of the group, so that
+// a rotation pair lies in one lane, each load is 16 bytes, and the row's cosines
+// and sines, the same for every head, are read once a wave. The sum of squares is
+// the lane's 16 squares, then a butterfly over the TH lanes.
+//
+// What bounds it is memory: each row read and written once. heads: units of a wave
+// (all of a row's where rows fill the chip, else one group a wave).
 template <int HD, bool BF>
 __global__ __launch_bounds__(256) void paged_prep_kernel(const uint16_t *qkv, int row_stride, uint16_t *q_out,
                                                          int q_stride, const float *__restrict__ qn,
                                                          const float *__restrict__ kn, const float *__restrict__ cs,
-                                                         int rope_rows, PagedView kv, int nh, int rot, float eps) {
-  constexpr int E = HD / 64;
-  const int head = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = blockIdx.x;
-  const int l = threadIdx.x & 63, nkv = kv.nkv, kvd = nkv * HD;
-  if (head >= nh + 2 * nkv) return;
+                                                         int rope_rows, PagedView kv, int nh, int rot, float eps, int T,
+                                                         int turns, int vec) {
+  constexpr int TH = HD / 16, U = 64 / TH;   // lanes a head, heads a turn
+  const int lane = threadIdx.x & 63, u = lane / TH, c = lane % TH;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nkv = kv.nkv, kvd = nkv * HD, heads = nh + 2 * nkv;
+  const int parts = (heads + U * turns - 1) / (U * turns);   // waves a row
+  const long long id = (long long)blockIdx.x * 4 + w;
+  const int row = (int)(id / parts), h0 = (int)(id % parts) * U * turns;
+  if (row >= T) return;
   int first, count;
   const int b = paged_seq_of_row(kv, row, first, count);
   if (b < 0) return;
-  const int pos = kv.kv_len[b] - count + (row - first);
+  const int pos = paged_len(kv, b) - count + (row - first);
   if (pos < 0 || pos >= rope_rows) return;
-  const uint16_t *xr = qkv + (size_t)row * row_stride + head * HD;
-  float x[E], r[E];
+  const long long at = paged_row(kv, b, pos, kvd);
+  const int half = rot / 2;
+  // the cosines and sines of this lane's pairs; 1 and 0 past the rotated dims
+  float co[8], si[8];
 #pragma unroll
-  for (int e = 0; e < E; e++) r[e] = x[e] = bf2f(xr[l + 64 * e]);
-  if (head < nh + nkv) {
-    const float *w = head < nh ? qn : kn;
-    float ss = 0.0f;
+  for (int i = 0; i < 8; i++) co[i] = 1.0f, si[i] = 0.0f;
+  const float *cr = cs + (size_t)pos * rot + 16 * c;
+  if (vec && 8 * c + 8 <= half) {
 #pragma unroll
-    for (int e = 0; e < E; e++) ss = __builtin_fmaf(x[e], x[e], ss);
-    const float rs = 1.0f / sqrtf(wave_pairwise_sum(ss) * (1.0f / (float)HD) + eps);
+    for (int i = 0; i < 8; i += 2) {
+      const float4 v = *reinterpret_cast<const float4 *>(cr + 2 * i);
+      co[i] = v.x, si[i] = v.y, co[i + 1] = v.z, si[i + 1] = v.w;
+    }
+  } else {
 #pragma unroll
-    for (int e = 0; e < E; e++) r[e] = w[l + 64 * e] * (x[e] * rs);
-    const int half = rot / 2;
-    const float *c = cs + (size_t)pos * rot;
-    if constexpr (HD == 64) {
-      const float other = __shfl_xor(r[0], 32, 64);
-      const int i = l & 31;
-      if (i < half) r[0] = r[0] * c[2 * i] + (l < 32 ? -other : other) * c[2 * i + 1];
-    } else if (l < half) {
-      const float a = r[0], b2 = r[1];
-      r[0] = a * c[2 * l] - b2 * c[2 * l + 1];
-      r[1] = b2 * c[2 * l] + a * c[2 * l + 1];
+    for (int i = 0; i < 8; i++)
+      if (8 * c + i < half) co[i] = cr[2 * i], si[i] = cr[2 * i + 1];
+  }
+  float wq[2][8], wk[2][8];
+#pragma unroll
+  for (int e = 0; e < 2; e++) {
+    const float *a = qn + e * (HD / 2) + 8 * c, *d = kn + e * (HD / 2) + 8 * c;
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        const float4 va = *reinterpret_cast<const float4 *>(a + i), vd = *reinterpret_cast<const float4 *>(d + i);
+        wq[e][i] = va.x, wq[e][i + 1] = va.y, wq[e][i + 2] = va.z, wq[e][i + 3] = va.w;
+        wk[e][i] = vd.x, wk[e][i + 1] = vd.y, wk[e][i + 2] = vd.z, wk[e][i + 3] = vd.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) wq[e][i] = a[i], wk[e][i] = d[i];
     }
   }
-  if (head < nh) {
+  for (int t = 0; t < turns; t++) {
+    const int head = h0 + t * U + u;
+    if (h0 + t * U >= heads) break;
+    const bool on = head < heads, norm = head < nh + nkv;
+    const uint16_t *xr = qkv + (size_t)row * row_stride + (on ? head : 0) * HD + 8 * c;
+    uint32_t xw[2][4];
 #pragma unroll
-    for (int e = 0; e < E; e++) q_out[(size_t)row * q_stride + head * HD + l + 64 * e] = f2bf(r[e]);
-    return;
+    for (int e = 0; e < 2; e++) {
+      if (vec) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(xr + e * (HD / 2));
+        xw[e][0] = v.x, xw[e][1] = v.y, xw[e][2] = v.z, xw[e][3] = v.w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) xw[e][i] = xr[e * (HD / 2) + 2 * i] | (uint32_t)xr[e * (HD / 2) + 2 * i + 1] << 16;
+      }
+    }
+    float x[2][8], ss = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        x[e][i] = __uint_as_float(i & 1 ? xw[e][i >> 1] & 0xffff0000u : xw[e][i >> 1] << 16);
+        ss = __builtin_fmaf(x[e][i], x[e][i], ss);
+      }
+    ss += dpp_f<kDppXor1>(ss);
+    ss += dpp_f<kDppXor2>(ss);
+    if constexpr (TH == 8) ss += dpp_f<kDppHalfMirror>(ss);
+    if (norm) {
+      const float rs = 1.0f / sqrtf(ss * (1.0f / (float)HD) + eps);
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const float a = (head < nh ? wq[0][i] : wk[0][i]) * (x[0][i] * rs), d = (head < nh ? wq[1][i] : wk[1][i]) * (x[1][i] * rs);
+        x[0][i] = a * co[i] - d * si[i];
+        x[1][i] = d * co[i] + a * si[i];
+      }
+    }
+    if (!on) continue;
+    const int g = head < nh + nkv ? head - nh : head - nh - nkv;
+    if (head >= nh && at < 0) continue;
+    uint16_t *dst = head < nh ? q_out + (size_t)row * q_stride + head * HD : (norm ? kv.k : kv.v) + at + g * HD;
+    const bool wide = head >= nh || vec;
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      uint32_t y[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float a = x[e][2 * i], d = x[e][2 * i + 1];
+        y[i] = head < nh || BF ? f2bf2(a, d) : (uint32_t)f2h(a) | (uint32_t)f2h(d) << 16;
+      }
+      uint16_t *to = dst + e * (HD / 2) + 8 * c;
+      if (wide) {
+        *reinterpret_cast<uint4 *>(to) = make_uint4(y[0], y[1], y[2], y[3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) to[2 * i] = (uint16_t)y[i], to[2 * i + 1] = (uint16_t)(y[i] >> 16);
+      }
+    }
   }
-  const long long at = paged_row(kv, b, pos, kvd);
-  if (at < 0) return;
-  const int g = head < nh + nkv ? head - nh : head - nh - nkv;
-  uint16_t *dst = (head < nh + nkv ? kv.k : kv.v) + at + g * HD;
-#pragma unroll
-  for (int e = 0; e < E; e++) dst[l + 64 * e] = BF ? f2bf(r[e]) : f2h(r[e]);
 }
 
 }  // namespace pq
@@ -120,10 +189,17 @@ extern "C" int pq_paged_qk_prep(const uint16_t *qkv, int row_stride, uint16_t *q
   PQ_REQUIRE(q_out != qkv || q_stride == row_stride, PQ_ERR_ARG, "pq_paged_qk_prep: q in place needs one row stride");
   PQ_REQUIRE(kv->q_start || T == kv->nseq, PQ_ERR_ARG, "pq_paged_qk_prep: %d rows for %d sequences without q_start", T,
              kv->nseq);
-  const dim3 grid(T, (nh + 2 * v.nkv + 3) / 4), block(256);
+  // 16-byte loads and stores of whole lanes where the rows allow it (the pools always do)
+  const int vec = aligned(qkv, 16) && row_stride % 8 == 0 && aligned(q_out, 16) && q_stride % 8 == 0 &&
+                  aligned(rope_cs, 16) && rot % 4 == 0 && aligned(q_norm, 16) && aligned(k_norm, 16);
+  const int heads = nh + 2 * v.nkv, U = 64 / (kv->hd / 16), groups = (heads + U - 1) / U;
+  const int turns = (long long)T * groups > 8192 ? groups : 1;
+  const long long waves = (long long)T * ((heads + U * turns - 1) / (U * turns));
+  PQ_REQUIRE((waves + 3) / 4 <= 1 << 24, PQ_ERR_ARG, "pq_paged_qk_prep: %d rows of %d heads are too many for one call", T, heads);
+  const dim3 grid((unsigned)((waves + 3) / 4)), block(256);
 #define PQ_PREP(HH, BB)                                                                                              \
   launch(paged_prep_kernel<HH, BB>, grid, block, 0, as_stream(stream), qkv, row_stride, q_out, q_stride, q_norm, k_norm, \
-         rope_cs, rope_rows, v, nh, rot, eps)
+         rope_cs, rope_rows, v, nh, rot, eps, T, turns, vec)
   const bool bf = kv->dtype == PQ_DTYPE_BF16;
   if (kv->hd == 64) {
     if (bf) PQ_PREP(64, true);
