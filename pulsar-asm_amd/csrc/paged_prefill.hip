@@ -90,7 +90,7 @@ struct PrefillArgs {
 // Grid (row tiles x kv heads, splits). Slot s of the row tiles: sequence b has the
 // slots from floor(q_start[b] G / BM) + b on, one more than it can need at most.
 template <int HD, bool BF, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void paged_prefill_kernel(PrefillArgs A, PagedView kv, int slots) {
+__global__ __launch_bounds__(64 * NW, HD == 64 && NW == 4 ? 3 : 2) void paged_prefill_kernel(PrefillArgs A, PagedView kv, int slots) {
   constexpr int BM = 32 * NW, S = HD / 16, N = HD / 32, RB = HD * 2;       // rows, score steps, dim tiles, bytes a row
   constexpr int TB = kKeys * RB, RPI = 1024 / RB, LI = TB / 1024 / NW;     // bytes a tile, rows and a wave's loads
   static_assert(LI >= 1, "a wave loads whole pieces");
@@ -100,21 +100,27 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_prefill_kernel(PrefillArgs A
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = blockIdx.x % kv.nkv, slot = slots - 1 - blockIdx.x / kv.nkv;
   const int G = A.G, kvd = kv.nkv * HD;
-  // the sequence of the slot
-  int b = -1;
+  // the sequence of the slot, its rows and its length: lane j reads sequence i + j's, the last one that starts at the
+  // slot or before is taken
+  int b = -1, q0 = 0, q1 = 0, len = 0;
   for (int i = 0; i < kv.nseq; i += 64) {
-    const int j = i + lane;
-    const int first = j < kv.nseq ? (kv.q_start != nullptr ? kv.q_start[j] : j) : 0x7fffffff;
+    const int j = i + lane, jc = j < kv.nseq ? j : kv.nseq - 1;
+    const int first = kv.q_start != nullptr ? kv.q_start[jc] : jc, next = kv.q_start != nullptr ? kv.q_start[jc + 1] : jc + 1;
+    const int n = paged_len(kv, jc);
     const int at = j < kv.nseq ? (first > 0 ? (int)((long long)first * G / BM) : 0) + j : 0x7fffffff;
-    b += __popcll(__ballot(at <= slot));
+    const int before = __popcll(__ballot(at <= slot));
+    if (before == 0) break;
+    b = i + before - 1;
+    q0 = __builtin_amdgcn_readlane(first, before - 1);
+    q1 = __builtin_amdgcn_readlane(next, before - 1);
+    len = __builtin_amdgcn_readlane(n, before - 1);
   }
   if (b < 0) return;
-  const int q0 = kv.q_start != nullptr ? kv.q_start[b] : b, q1 = kv.q_start != nullptr ? kv.q_start[b + 1] : b + 1;
   if (q0 < 0 || q1 > A.T || q1 <= q0) return;
   const int rows = (q1 - q0) * G, r0 = (slot - ((int)((long long)q0 * G / BM) + b)) * BM;
   if (r0 >= rows) return;
   // positions: row i of the sequence is at p0 + i
-  const int p0 = paged_len(kv, b) - (q1 - q0);
+  const int p0 = len - (q1 - q0);
   const int rlast = r0 + BM < rows ? r0 + BM - 1 : rows - 1;
   const int pmin = p0 + r0 / G, pmax = p0 + rlast / G;
   const int limit = pmax + 1 < kv.cap ? pmax + 1 : kv.cap;                 // keys from here on are no row's

@@ -489,6 +489,7 @@ class PagedKV:
         if any(t.device != k.device for t in (v, *ints)):
             raise ValueError("the pools, the table and the lengths must be on one device")
         self.tensors = (k, v, table, kv_len, q_start)   # kept alive with the view
+        self.needs = {}                                 # workspace bytes by a call's sizes
         self.npages, self.page, self.nkv, self.hd, self.nseq = npages, page, nkv, hd, nseq
         self.capacity = table.shape[1] * page
         self.device = k.device
@@ -504,9 +505,10 @@ class PagedKV:
 
 def _paged_rows(kv, what, t, width):
     """Rows [T][>= width] of 16-bit storage on the view's device: (pointer, row stride, T)."""
-    if t.dtype not in _RAW16 or t.dim() != 2 or t.shape[1] < width or t.stride(1) != 1 or t.device != kv.device:
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[1] < width or stride[1] != 1 or t.dtype not in _RAW16 or t.device != kv.device:
         raise ValueError(f"{what} must be bf16 rows of at least {width} on the cache's device, unit column stride")
-    return t.data_ptr(), t.stride(0), t.shape[0]
+    return t.data_ptr(), stride[0], shape[0]
 
 
 def _paged_stream(kv):
@@ -563,12 +565,19 @@ def _paged_attn(kv, q, nh, scale, gate, win, sinks, max_kv, out, qx, dx, ws, pre
     if max_kv is None:
         max_kv = kv.capacity
     L = lib()
-    if prefill:
-        need = L.pq_paged_prefill_workspace_bytes(kv.nseq, T, nh, kv.nkv, kv.hd, max_kv, win, sinks)
-    else:
-        need = L.pq_paged_decode_workspace_bytes(kv.nseq, nh, kv.nkv, kv.hd, max_kv, win, sinks)
-    if need and ws is None:
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    if ws is None:
+        sizes = (prefill, T, nh, max_kv, win, sinks)
+        need = kv.needs.get(sizes)
+        if need is None:
+            need = L.pq_paged_prefill_workspace_bytes(kv.nseq, T, nh, kv.nkv, kv.hd, max_kv, win, sinks) if prefill else \
+                L.pq_paged_decode_workspace_bytes(kv.nseq, nh, kv.nkv, kv.hd, max_kv, win, sinks)
+            if len(kv.needs) > 4096:
+                kv.needs.clear()
+            kv.needs[sizes] = need
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif ws.device != kv.device or not ws.is_contiguous():
+        raise ValueError("ws must be contiguous on the cache's device")
     wp, wn = (ws.data_ptr(), ws.numel() * ws.element_size()) if ws is not None else (None, 0)
     st = _paged_stream(kv)
     if prefill:
