@@ -566,6 +566,8 @@ int pq_paged_qk_prep(const uint16_t *qkv, int row_stride, uint16_t *q_out, int q
  * max_kv: about the largest kv_len (it sets how far the work is split, and
  * the workspace with it; any length is computed whole). The keys are split over
  * workgroups and joined in a fixed order: the same call gives the same bits.
+ * out must not overlap q. Weights are rounded to 16 bits of mantissa (fp16: 11)
+ * for the value product, everything else is fp32.
  * ws (16-byte aligned): pq_paged_decode_workspace_bytes, 0 where one workgroup
  * a kv head does it. */
 size_t pq_paged_decode_workspace_bytes(int nseq, int nh, int nkv, int hd, int max_kv, int win, int sinks);
@@ -576,7 +578,7 @@ int pq_paged_attn_decode(const uint16_t *q, int q_stride, const pq_paged_kv *kv,
 /* The same for prompt rows: T rows of a ragged batch (kv->q_start), each row
  * at its position p, with the keys of the sequence's earlier rows in the pages
  * (pq_paged_qk_prep of the batch before it). Rows outside the sequences keep
- * what they held. */
+ * what they held. Weights are rounded to the pool's type for the value product. */
 size_t pq_paged_prefill_workspace_bytes(int nseq, int T, int nh, int nkv, int hd, int max_kv, int win, int sinks);
 int pq_paged_attn_prefill(const uint16_t *q, int q_stride, const pq_paged_kv *kv, const uint16_t *gate,
                           int gate_stride, uint16_t *out, int out_stride, int8_t *qx, float *dx, int nh, int T,

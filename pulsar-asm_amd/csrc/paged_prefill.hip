@@ -118,7 +118,7 @@ __global__ __launch_bounds__(64 * NW, HD == 64 && NW == 4 ? 3 : 2) void paged_pr
   if (b < 0) return;
   if (q0 < 0 || q1 > A.T || q1 <= q0) return;
   const int rows = (q1 - q0) * G, r0 = (slot - ((int)((long long)q0 * G / BM) + b)) * BM;
-  if (r0 >= rows) return;
+  if (r0 < 0 || r0 >= rows) return;   // below 0: q_start does not ascend
   // positions: row i of the sequence is at p0 + i
   const int p0 = len - (q1 - q0);
   const int rlast = r0 + BM < rows ? r0 + BM - 1 : rows - 1;

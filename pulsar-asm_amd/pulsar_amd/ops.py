@@ -458,6 +458,7 @@ def attn_layer_decode(qkvg, q_norm, k_norm, rope_cs, kc, vc, pos, nh, nkv, hd, r
 # --------------------------------------------------------------- paged cache
 _DT_OF = {torch.float16: 2, torch.bfloat16: 1}
 _RAW16 = (torch.bfloat16, torch.int16, torch.uint16)
+_INT_MAX = 2 ** 31 - 1
 
 
 class PagedKV:
@@ -491,7 +492,7 @@ class PagedKV:
         self.tensors = (k, v, table, kv_len, q_start)   # kept alive with the view
         self.needs = {}                                 # workspace bytes by a call's sizes
         self.npages, self.page, self.nkv, self.hd, self.nseq = npages, page, nkv, hd, nseq
-        self.capacity = table.shape[1] * page
+        self.capacity = min(table.shape[1] * page, _INT_MAX)
         self.device = k.device
         self.index = k.device.index if k.device.type == "cuda" else None
         c = self.c = PagedKVView()
@@ -564,6 +565,8 @@ def _paged_attn(kv, q, nh, scale, gate, win, sinks, max_kv, out, qx, dx, ws, pre
         raise ValueError("qx must be int8 [T][nh * hd], dx fp32 [T][nh * hd / 32], contiguous on the cache's device")
     if max_kv is None:
         max_kv = kv.capacity
+    if not (0 <= win <= _INT_MAX and 0 <= sinks <= _INT_MAX and 0 < max_kv <= _INT_MAX and nh <= _INT_MAX):
+        raise ValueError("win, sinks and max_kv must fit an int, max_kv above 0")
     L = lib()
     if ws is None:
         sizes = (prefill, T, nh, max_kv, win, sinks)

@@ -242,6 +242,20 @@ def test_decode_offsets_past_32_bits(pq, dev):
     assert torch.equal(big_v[int(table[0, 500 // page]), 500 % page], v)
 
 
+def test_decode_many_sequences(pq, dev):
+    """More sequences than the split's threads, lengths from none to long, both ways of laying the call out."""
+    past = [(37 * i) % 190 for i in range(300)]
+    past[123], past[299] = 1700, 2500
+    for nh, nkv, hd, cache in ((8, 8, 64, F16), (4, 1, 128, BF16)):
+        bt = pc.Batch(dev, [1] * 300, past, nh, nkv, hd, 16, cache, seed=13)
+        for win, sinks in ((0, 0), (64, 2)):
+            want, tol = pc.want(bt, 0.1, win, sinks)
+            for hint in (64, None):
+                print(f"decode 300 {nh}/{nkv}x{hd} win={win} hint={hint}", flush=True)
+                pc.check(pq.paged_attn_decode(bt.view(pq, False), bt.rows, nh, 0.1, gate=bt.gate, win=win, sinks=sinks,
+                                              max_kv=hint), want, tol)
+
+
 # ------------------------------------------------------------------ prompt rows
 PREFILL = [
     (32, 8, 64, F16, 16, [1], [0], 0, 0, {}),
@@ -328,6 +342,52 @@ def test_prefill_empty_rows_and_bad_pages(pq, dev):
     bt.kv_len[1] = 25
     got = pq.paged_attn_prefill(bt.view(pq), bt.rows, nh, 0.09)
     assert (got[20:35] == 0).all() and torch.isfinite(got[35:60]).all() and (got[35:60] != 0).any()
+
+
+def test_prefill_many_sequences_and_one_row_each(pq, dev):
+    """More sequences than a wave's lanes; and without q_start: a row a sequence, as the decode call."""
+    nh, nkv, hd = 8, 2, 64
+    q, past = [(7 * i) % 23 for i in range(150)], [(31 * i) % 170 for i in range(150)]
+    bt = pc.Batch(dev, q, past, nh, nkv, hd, 16, F16, seed=32)
+    want, tol = pc.want(bt, 0.1, 0, 0)
+    pc.check(pq.paged_attn_prefill(bt.view(pq), bt.rows, nh, 0.1, gate=bt.gate), want, tol)
+    bt = pc.Batch(dev, [1] * 150, past, nh, nkv, hd, 16, F16, seed=33)
+    want, tol = pc.want(bt, -0.1, 90, 3)
+    for hint in (20, 4000):
+        pc.check(pq.paged_attn_prefill(bt.view(pq, False), bt.rows, nh, -0.1, gate=bt.gate, win=90, sinks=3, max_kv=hint),
+                 want, tol)
+        pc.check(pq.paged_attn_decode(bt.view(pq, False), bt.rows, nh, -0.1, gate=bt.gate, win=90, sinks=3, max_kv=hint),
+                 want, tol)
+
+
+@pytest.mark.parametrize("cache,hd", [(F16, 64), (BF16, 128)])
+def test_scale_of_zero(pq, dev, cache, hd):
+    """Every visible key has one weight."""
+    bt = pc.Batch(dev, [70, 1], [30, 200], 8, 2, hd, 16, cache, seed=34)
+    want, tol = pc.want(bt, 0.0, 40, 2)
+    pc.check(pq.paged_attn_prefill(bt.view(pq), bt.rows, 8, 0.0, gate=bt.gate, win=40, sinks=2), want, tol)
+    one = pq.PagedKV(bt.k, bt.v, bt.table[1:], bt.kv_len[1:])
+    pc.check(pq.paged_attn_decode(one, bt.rows[70:], 8, 0.0, gate=bt.gate[70:], win=40, sinks=2), want[70:], tol[70:])
+
+
+def test_row_starts_that_do_not_ascend(pq, dev):
+    """Such a sequence has no rows: the others' are right, and nothing else is written."""
+    nh, nkv, hd = 8, 2, 64
+    bt = pc.Batch(dev, [40, 30, 20], [10, 50, 0], nh, nkv, hd, 16, F16, seed=35)
+    want, tol = pc.want(bt, 0.1, 0, 0)
+    kv = bt.view(pq)
+    for starts in ([0, 40, 10, 20], [90, 60, 30, 0], [-5, 40, 70, 200], [0, 1 << 30, 5, 90]):
+        print(starts, flush=True)
+        bt.q_start.copy_(torch.tensor(starts))
+        out = torch.full((bt.T + 8, nh * hd), 5.0, dtype=BF16, device=dev)
+        pq.paged_attn_prefill(kv, bt.rows, nh, 0.1, gate=bt.gate, out=out[4:-4])
+        pq.paged_qk_prep(kv, bt.rows, torch.ones(hd, device=dev), torch.ones(hd, device=dev),
+                         torch.ones((100, 16, 2), device=dev), nh, 32)
+        assert (out[:4] == 5).all() and (out[-4:] == 5).all()
+    torch.cuda.synchronize()
+    bt.q_start.copy_(torch.tensor(bt.starts))
+    bt.store()
+    pc.check(pq.paged_attn_prefill(kv, bt.rows, nh, 0.1, gate=bt.gate), want, tol)
 
 
 # --------------------------------------------------------------------- together

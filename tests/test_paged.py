@@ -111,7 +111,8 @@ def test_call_refusals():
     for call in (pq.paged_attn_decode, pq.paged_attn_prefill):
         for bad in (dict(q=rows.float()), dict(q=rows[:, :2040]), dict(gate=rows[:1, :32]), dict(gate=rows[:, :31]),
                     dict(out=rows[:, :2040]), dict(out=rows[:1]), dict(qx=qx), dict(qx=qx, dx=dx.half()),
-                    dict(qx=qx[:, :64], dx=dx), dict(qx=qx.float(), dx=dx)):
+                    dict(qx=qx[:, :64], dx=dx), dict(qx=qx.float(), dx=dx), dict(win=-1), dict(sinks=-1), dict(win=2 ** 32),
+                    dict(max_kv=0), dict(max_kv=2 ** 31), dict(ws=torch.zeros(8, 8)[:, :4])):
             kw = dict(q=rows)
             kw.update(bad)
             with pytest.raises(ValueError):
