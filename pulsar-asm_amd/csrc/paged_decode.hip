@@ -22,7 +22,7 @@
 // Each tile's loads run a tile ahead of its use in the same registers.
 //
 // Measured: 131072 keys of 4 kv heads of 128, one sequence 58 us (268 MB, 4.6 TB/s with
-// the join's 9 us), 64 sequences of up to 8192 keys of 8 heads of 64 112 us (563 MB, 5.0),
+// the join's 7 us), 64 sequences of up to 8192 keys of 8 heads of 64 112 us (563 MB, 5.0),
 // 256 windows of 260 keys of 4 heads of 128 34 us (137 MB, 4.1), 300 keys 9.6 us, the
 // call's host time; a plain read of those bytes takes 38, 80 and 20 us.
 #include <type_traits>
