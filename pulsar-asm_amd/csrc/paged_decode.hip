@@ -21,8 +21,8 @@
 // Heads past G are zero columns: the matrix cores have 25 times the work's rate.
 // Each tile's loads run a tile ahead of its use in the same registers.
 //
-// Measured: 131072 keys of 4 kv heads of 128, one sequence 58 us (268 MB, 4.6 TB/s with
-// the join's 7 us), 64 sequences of up to 8192 keys of 8 heads of 64 112 us (563 MB, 5.0),
+// Measured: 131072 keys of 4 kv heads of 128, one sequence 56 us (268 MB, 4.8 TB/s with
+// the join's 7 us), 64 sequences of up to 8192 keys of 8 heads of 64 102 us (563 MB, 5.5),
 // 256 windows of 260 keys of 4 heads of 128 34 us (137 MB, 4.1), 300 keys 9.6 us, the
 // call's host time; a plain read of those bytes takes 38, 80 and 20 us.
 #include <type_traits>
@@ -75,6 +75,13 @@ __device__ __forceinline__ v4f mfma16(v4u a, v4u b, v4f c) {
 
 __device__ __forceinline__ uint32_t f2h2(float a, float b) { return (uint32_t)f2h(a) | (uint32_t)f2h(b) << 16; }
 
+// a piece of K or V; NT: not to be kept in the caches
+template <bool NT, typename T>
+__device__ __forceinline__ T read_kv(const uint16_t *p) {
+  if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const T *>(p));
+  else return *reinterpret_cast<const T *>(p);
+}
+
 // A workgroup's 4 waves are HW kv heads (a group) by KW = 4 / HW ways through the
 // keys. A segment is a group of one sequence, its work the sequence's tiles.
 //
@@ -88,7 +95,7 @@ __device__ __forceinline__ uint32_t f2h2(float a, float b) { return (uint32_t)f2
 // l < 0: no key. seg[]: where the segments are cut: by_wg, entry x is the segment whose
 // first piece is part 2 x + 1 (-1: none) and its last workgroup; else entry
 // (sequence, group) is the segment's first and last workgroup.
-template <int HD, bool BF>
+template <int HD, bool BF, bool NT>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_split_kernel(
     const uint16_t *__restrict__ q, int q_stride, int qvec, PagedView kv, const uint16_t *__restrict__ gate,
     int gate_stride, uint16_t *__restrict__ out, int out_stride, int8_t *__restrict__ qx, float *__restrict__ dx, int nh,
@@ -183,7 +190,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_split_kernel(
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
-              for (int s = 0; s < S; s++) kw[u][s] = *reinterpret_cast<const v4u *>(kr + 4 * u * kvd + 32 * s);
+              for (int s = 0; s < S; s++) kw[u][s] = read_kv<NT, v4u>(kr + 4 * u * kvd + 32 * s);
           };
           auto load_v = [&](int i) {
             const int jv = paged_tile_base(t, i) + 8 * Q;
@@ -192,10 +199,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_split_kernel(
 #pragma unroll
             for (int j = 0; j < 8; j++) {
               if constexpr (VW == 4) {
-                const v4u x = *reinterpret_cast<const v4u *>(vr + (size_t)j * kvd);
+                const v4u x = read_kv<NT, v4u>(vr + (size_t)j * kvd);
                 vw[j][0] = x[0], vw[j][1] = x[1], vw[j][2] = x[2], vw[j][3] = x[3];
               } else {
-                const v2u x = *reinterpret_cast<const v2u *>(vr + (size_t)j * kvd);
+                const v2u x = read_kv<NT, v2u>(vr + (size_t)j * kvd);
                 vw[j][0] = x[0], vw[j][1] = x[1];
               }
             }
@@ -552,14 +559,22 @@ __global__ __launch_bounds__(kJoin) void paged_join_kernel(const uint16_t *__res
 // keys, the longer each and the better memory answers (64 sequences of 8192 keys of 8
 // heads of 64: 8 workgroups a CU in pieces of 256 keys 4.8 TB/s, one a CU 5.7). One a CU for
 // head_dim 128 (131072 keys of 4 heads 58.4 us, two a CU 63.5), two for 64 (64
-// sequences of up to 8192 112.4, one a CU 113.2, 128 of up to 600 32.5 / 36.1).
+// sequences of up to 8192 112.4, one a CU 113.2, 128 of up to 600 32.5 / 36.1; all of
+// these before the reads past the caches below).
+//
+// K and V are read past the caches (once) where they fill the last-level cache of 256
+// MiB, as nothing of them is left there for the next call: 563 MB 112 -> 102 us, 268 MB
+// 58.4 -> 56.2, 128 sequences of up to 4800 keys of 8 heads of 64 151 -> 139; below that a pool
+// that is read again finds some of it there (32 sequences of 1200, 50 MB, 15.8 / 21.8).
 struct PagedPlan {
   int HW, grid, share, by_wg;
+  bool once;
 };
 static PagedPlan paged_plan(int nseq, int nkv, int hd, int max_kv, int win, int sinks) {
   const int tiles = paged_tiles(max_kv, 0x7fffffff, win, sinks).count;
   const bool even = tiles > 40;
-  PagedPlan p = {1, 1, 0, 0};
+  PagedPlan p = {1, 1, 0, 0, false};
+  p.once = (long long)nseq * nkv * tiles * (kTile * 4LL) * hd >= 256LL << 20;
   p.HW = even ? 4 : (long long)nseq * nkv >= 1024 ? 2 : 1;
   while (nkv % p.HW) p.HW >>= 1;
   const long long segs = (long long)nseq * (nkv / p.HW);
@@ -615,9 +630,15 @@ extern "C" int pq_paged_attn_decode(const uint16_t *q, int q_stride, const pq_pa
   const int qvec = aligned(q, 16) && q_stride % 8 == 0 ? 1 : 0;
   hipStream_t st = as_stream(stream);
   const size_t lds = (size_t)kWaves * G * (hd + 4) * sizeof(float);
-#define PQ_SPLIT(HH, BB)                                                                                              \
-  launch(paged_split_kernel<HH, BB>, dim3(p.grid), dim3(64 * kWaves), lds, st, q, q_stride, qvec, v, gate, gate_stride, \
-         out, out_stride, qx, dx, nh, G, scale, win, sinks, p.HW, p.share, p.by_wg, po, pml, seg)
+#define PQ_SPLIT(HH, BB)                                                                                           \
+  do {                                                                                                             \
+    if (p.once)                                                                                                    \
+      launch(paged_split_kernel<HH, BB, true>, dim3(p.grid), dim3(64 * kWaves), lds, st, q, q_stride, qvec, v, gate, \
+             gate_stride, out, out_stride, qx, dx, nh, G, scale, win, sinks, p.HW, p.share, p.by_wg, po, pml, seg);  \
+    else                                                                                                           \
+      launch(paged_split_kernel<HH, BB, false>, dim3(p.grid), dim3(64 * kWaves), lds, st, q, q_stride, qvec, v, gate, \
+             gate_stride, out, out_stride, qx, dx, nh, G, scale, win, sinks, p.HW, p.share, p.by_wg, po, pml, seg);  \
+  } while (0)
   const bool bf = kv->dtype == PQ_DTYPE_BF16;
   if (hd == 64) {
     if (bf) PQ_SPLIT(64, true);
