@@ -557,7 +557,7 @@ int pq_paged_qk_prep(const uint16_t *qkv, int row_stride, uint16_t *q_out, int q
 /* Attention of one new token a sequence over its pages: row b of q (bf16,
  * q_stride elements a row) at position p = kv_len[b] - 1 (q_start is not read)
  * sees the keys j <= p with win == 0, or j > p - win, or j < sinks: a sliding
- * window whose first `sinks` tokens stay visible. nh / nkv is any whole number
+ * window (at most 2^30) whose first `sinks` tokens stay visible. nh / nkv is any whole number
  * up to 16. s_j = scale * q . k_j, o = sum e^(s_j - max) v_j / sum e^(s_j - max);
  * out (bf16, out_stride elements a row) = o * sigmoid(gate[b][head]) (gate NULL
  * for none), rounded once, and/or its Q8_0 form (qx [nseq][nh hd], dx, as

@@ -87,7 +87,7 @@ __device__ __forceinline__ T read_kv(const uint16_t *p) {
 //
 // share == 0: a workgroup a segment, which writes the output. share > 0: the
 // segments' tiles lie end to end in order of (sequence, group) and workgroup x
-// takes the tiles [x c, (x + 1) c), c = max(total / gridDim, share), so that all
+// takes the tiles [x per, (x + 1) per), per = max(total / gridDim + 1, share), so that all
 // carry the same work whatever the lengths. A segment that lies whole in one
 // workgroup's tiles is output at once; of one cut in pieces, a workgroup holds at
 // most two (its first, which began in the workgroup before, and its last): part
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_split_kernel(
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int w = wave / HW;
   const int kvd = kv.nkv * HD;
-  // the workgroup's tiles [at, end); b, gg, base: the segment that holds `at`, and where it begins
+  // the workgroup's tiles [at, end); b, gg, begin: the segment that holds `at`, and where it begins
   int b, gg;
   long long at, end, begin, per = 0;
   if (share == 0) {
@@ -172,42 +172,42 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_split_kernel(
     const int slots = (1 << kv.lg_page) - 1;
     // the page of 8 keys from j: a lane's K keys lie in group c / 4 of the tile, its V keys in group Q
     auto page_of = [&](int j) { return j < t.n ? tb[j >> kv.lg_page] : -1; };
-          // the tile's loads run a tile ahead: K's as soon as the scores have read the registers, V's after the value
-          // products, the page ids two tiles ahead
-          v4u kw[2][S];
-          uint32_t vw[8][VW];
-          int idk = -1, idv = -1, pgk = -1, pgv = -1;
-          auto ids = [&](int i) {
-            if (i >= t1) return;
-            const int base = paged_tile_base(t, i);
-            idk = page_of(base + 8 * (c >> 2));
-            idv = page_of(base + 8 * Q);
-          };
-          auto load_k = [&](int i) {
-            const int jk = paged_tile_base(t, i) + 8 * (c >> 2);
-            const bool ok = (unsigned)pgk < (unsigned)kv.npages;
-            const uint16_t *kr = kv.k + (ok ? pgk : 0) * kv.page_stride + (long long)((jk & slots) + (c & 3)) * kvd + g * HD + 8 * Q;
+    // the tile's loads run a tile ahead: K's as soon as the scores have read the registers, V's after the value
+    // products, the page ids two tiles ahead
+    v4u kw[2][S];
+    uint32_t vw[8][VW];
+    int idk = -1, idv = -1, pgk = -1, pgv = -1;
+    auto ids = [&](int i) {
+      if (i >= t1) return;
+      const int base = paged_tile_base(t, i);
+      idk = page_of(base + 8 * (c >> 2));
+      idv = page_of(base + 8 * Q);
+    };
+    auto load_k = [&](int i) {
+      const int jk = paged_tile_base(t, i) + 8 * (c >> 2);
+      const bool ok = (unsigned)pgk < (unsigned)kv.npages;
+      const uint16_t *kr = kv.k + (ok ? pgk : 0) * kv.page_stride + (long long)((jk & slots) + (c & 3)) * kvd + g * HD + 8 * Q;
 #pragma unroll
-            for (int u = 0; u < 2; u++)
+      for (int u = 0; u < 2; u++)
 #pragma unroll
-              for (int s = 0; s < S; s++) kw[u][s] = read_kv<NT, v4u>(kr + 4 * u * kvd + 32 * s);
-          };
-          auto load_v = [&](int i) {
-            const int jv = paged_tile_base(t, i) + 8 * Q;
-            const bool ok = (unsigned)pgv < (unsigned)kv.npages;
-            const uint16_t *vr = kv.v + (ok ? pgv : 0) * kv.page_stride + (long long)(jv & slots) * kvd + g * HD + (HD / 16) * c;
+        for (int s = 0; s < S; s++) kw[u][s] = read_kv<NT, v4u>(kr + 4 * u * kvd + 32 * s);
+    };
+    auto load_v = [&](int i) {
+      const int jv = paged_tile_base(t, i) + 8 * Q;
+      const bool ok = (unsigned)pgv < (unsigned)kv.npages;
+      const uint16_t *vr = kv.v + (ok ? pgv : 0) * kv.page_stride + (long long)(jv & slots) * kvd + g * HD + (HD / 16) * c;
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-              if constexpr (VW == 4) {
-                const v4u x = read_kv<NT, v4u>(vr + (size_t)j * kvd);
-                vw[j][0] = x[0], vw[j][1] = x[1], vw[j][2] = x[2], vw[j][3] = x[3];
-              } else {
-                const v2u x = read_kv<NT, v2u>(vr + (size_t)j * kvd);
-                vw[j][0] = x[0], vw[j][1] = x[1];
-              }
-            }
-          };
-          auto start = [&]() {
+      for (int j = 0; j < 8; j++) {
+        if constexpr (VW == 4) {
+          const v4u x = read_kv<NT, v4u>(vr + (size_t)j * kvd);
+          vw[j][0] = x[0], vw[j][1] = x[1], vw[j][2] = x[2], vw[j][3] = x[3];
+        } else {
+          const v2u x = read_kv<NT, v2u>(vr + (size_t)j * kvd);
+          vw[j][0] = x[0], vw[j][1] = x[1];
+        }
+      }
+    };
+    auto start = [&]() {
       ids(t0 + w);
       pgk = idk;
       pgv = idv;

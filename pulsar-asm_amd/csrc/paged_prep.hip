@@ -42,7 +42,8 @@ int paged_attn_check(const char *who, const uint16_t *q, int q_stride, const pq_
   const int rc = paged_view(kv, who, v);
   if (rc) return rc;
   PQ_REQUIRE((long long)v->nseq * v->nkv <= 1 << 23, PQ_ERR_ARG, "%s: nseq=%d x nkv=%d (at most 2^23)", who, v->nseq, v->nkv);
-  PQ_REQUIRE(nh > 0 && nh % v->nkv == 0 && nh / v->nkv <= 16 && win >= 0 && sinks >= 0 && max_kv > 0, PQ_ERR_ARG,
+  PQ_REQUIRE(nh > 0 && nh % v->nkv == 0 && nh / v->nkv <= 16 && win >= 0 && win <= 1 << 30 && sinks >= 0 && max_kv > 0,
+             PQ_ERR_ARG,
              "%s: nh=%d nkv=%d win=%d sinks=%d max_kv=%d", who, nh, v->nkv, win, sinks, max_kv);
   PQ_REQUIRE(q_stride >= nh * kv->hd && (!out || out_stride >= nh * kv->hd) && (!gate || gate_stride >= nh), PQ_ERR_ARG,
              "%s: row strides %d, %d and %d too small", who, q_stride, out_stride, gate_stride);

@@ -565,8 +565,8 @@ def _paged_attn(kv, q, nh, scale, gate, win, sinks, max_kv, out, qx, dx, ws, pre
         raise ValueError("qx must be int8 [T][nh * hd], dx fp32 [T][nh * hd / 32], contiguous on the cache's device")
     if max_kv is None:
         max_kv = kv.capacity
-    if not (0 <= win <= _INT_MAX and 0 <= sinks <= _INT_MAX and 0 < max_kv <= _INT_MAX and nh <= _INT_MAX):
-        raise ValueError("win, sinks and max_kv must fit an int, max_kv above 0")
+    if not (0 <= win <= 1 << 30 and 0 <= sinks <= _INT_MAX and 0 < max_kv <= _INT_MAX and nh <= _INT_MAX):
+        raise ValueError("win must be 0 .. 2^30, sinks and max_kv must fit an int, max_kv above 0")
     L = lib()
     if ws is None:
         sizes = (prefill, T, nh, max_kv, win, sinks)

@@ -342,6 +342,9 @@ def test_prefill_empty_rows_and_bad_pages(pq, dev):
     bt.kv_len[1] = 25
     got = pq.paged_attn_prefill(bt.view(pq), bt.rows, nh, 0.09)
     assert (got[20:35] == 0).all() and torch.isfinite(got[35:60]).all() and (got[35:60] != 0).any()
+    # the widest window and as many sinks are no window
+    for kw in (dict(win=1 << 30), dict(win=1 << 30, sinks=2 ** 31 - 1), dict(sinks=2 ** 31 - 1)):
+        assert torch.equal(pq.paged_attn_prefill(bt.view(pq), bt.rows, nh, 0.09, **kw), got)
 
 
 def test_prefill_many_sequences_and_one_row_each(pq, dev):

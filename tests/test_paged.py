@@ -69,8 +69,8 @@ def test_rows_without_q_start():
 
 
 @pytest.mark.parametrize("bad", [
-    dict(q=None), dict(out=None), dict(qx=64), dict(nh=0), dict(nh=30), dict(nh=136), dict(win=-1), dict(sinks=-1),
-    dict(most=0), dict(qs=2047), dict(os=2047), dict(gs=31)])
+    dict(q=None), dict(out=None), dict(qx=64), dict(nh=0), dict(nh=30), dict(nh=136), dict(win=-1), dict(win=(1 << 30) + 1),
+    dict(sinks=-1), dict(most=0), dict(qs=2047), dict(os=2047), dict(gs=31)])
 def test_bad_attention(bad):
     for call in (_decode, _prefill):
         assert call(_view(), **bad) == ARG, (call.__name__, bad)
