@@ -6,6 +6,9 @@
 
 namespace pq {
 
+// positions that are counted of any table: leaves a tile's end room in an int
+constexpr int kPagedCap = 0x7fffff00;
+
 // pq_paged_kv as the kernels take it (by value). cap: positions a table row covers.
 struct PagedView {
   uint16_t *k, *v;

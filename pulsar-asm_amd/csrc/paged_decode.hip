@@ -39,18 +39,20 @@ constexpr int kTile = 32;     // keys of a wave's step
 constexpr int kWaves = 4;     // waves a workgroup
 
 // The tiles of a sequence of n positions: those of the sinks, then those of the window.
+// What the sinks reach is cut to the cap before it is rounded up, so that no length,
+// window or sink count wraps (cap <= kPagedCap).
 struct PagedTiles {
   int n, lo, ns, sink, first, count;
 };
 __host__ __device__ inline PagedTiles paged_tiles(int n, int cap, int win, int sinks) {
   PagedTiles t;
+  t.n = n < cap ? (n > 0 ? n : 0) : cap;
   t.lo = win > 0 && n > win ? n - win : 0;
   t.ns = sinks < t.lo ? sinks : t.lo;
-  t.n = n < cap ? n : cap;
+  if (t.ns > t.n) t.ns = t.n;
   t.sink = (t.ns + kTile - 1) / kTile;
   t.first = t.lo / kTile > t.sink ? t.lo / kTile : t.sink;
-  const int end = (int)(((long long)t.n + kTile - 1) / kTile);
-  if (t.sink > end) t.sink = end > 0 ? end : 0;
+  const int end = (t.n + kTile - 1) / kTile;
   t.count = t.sink + (end > t.first ? end - t.first : 0);
   return t;
 }
@@ -571,7 +573,7 @@ struct PagedPlan {
   bool once;
 };
 static PagedPlan paged_plan(int nseq, int nkv, int hd, int max_kv, int win, int sinks) {
-  const int tiles = paged_tiles(max_kv, 0x7fffffff, win, sinks).count;
+  const int tiles = paged_tiles(max_kv, kPagedCap, win, sinks).count;
   const bool even = tiles > 40;
   PagedPlan p = {1, 1, 0, 0, false};
   p.once = (long long)nseq * nkv * tiles * (kTile * 4LL) * hd >= 256LL << 20;

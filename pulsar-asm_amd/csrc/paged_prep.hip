@@ -31,7 +31,7 @@ int paged_view(const pq_paged_kv *kv, const char *who, PagedView *out) {
   out->nseq = kv->nseq;
   out->table_stride = kv->table_stride;
   const long long cap = (long long)kv->table_pages * kv->page;
-  out->cap = cap < 0x7fffff00LL ? (int)cap : 0x7fffff00;   // room for a tile's end in an int
+  out->cap = cap < kPagedCap ? (int)cap : kPagedCap;
   return PQ_OK;
 }
 

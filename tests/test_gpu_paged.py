@@ -534,3 +534,26 @@ def test_same_call_same_bits(pq, dev):
     for _ in range(3):
         assert torch.equal(pq.paged_attn_decode(a.view(pq, False), a.rows, 16, 0.09, gate=a.gate), wa)
         assert torch.equal(pq.paged_attn_prefill(b.view(pq), b.rows, 16, 0.09, gate=b.gate), wb)
+
+
+@pytest.mark.parametrize("cache,nh,nkv,hd", [(F16, 8, 2, 64), (BF16, 4, 1, 128)])
+def test_lengths_and_sinks_near_the_largest_int(pq, dev, cache, nh, nkv, hd):
+    """Lengths near 2^31, far past the table, with as many sinks: the keys of the table that the sinks reach are seen,
+    those of a window that lies past it are not."""
+    top = 2 ** 31 - 1
+    bt = pc.Batch(dev, [1, 1], [319, 63], nh, nkv, hd, 16, cache, seed=91)
+    for n in (top, top - 40, -top - 1):
+        bt.kv_len.fill_(n)
+        for win, sinks in ((1, top), (30, top), (1, 50), (30, 0), (0, 0), (1 << 30, top)):
+            print(n, win, sinks, flush=True)
+            table = bt.table.clone()
+            table[1, 4:] = -1
+            kv = pq.PagedKV(bt.k, bt.v, table, bt.kv_len)
+            for call in (pq.paged_attn_decode, pq.paged_attn_prefill):
+                for hint in (1, top):
+                    got = call(kv, bt.rows, nh, 0.1, win=win, sinks=sinks, max_kv=hint)
+                    for b in range(2):
+                        p = torch.tensor([n - 1], device=dev)
+                        o, size, slack = pc.attend64(bt.rows[b:b + 1, :nh * hd].view(1, nh, hd), p, bt.keys[b], bt.vals[b],
+                                                     0.1, win, sinks)
+                        pc.check(got[b:b + 1], o, pc.tolerance(o, size, slack, bt.n[b], cache))

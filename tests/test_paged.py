@@ -123,3 +123,17 @@ def test_call_refusals():
         pq.paged_attn_decode(kv, rows[:1], 32, 0.125)
     with pytest.raises(ValueError, match="GPU"):
         pq.paged_qk_prep(kv, rows, w, w, cs, 32, 32)
+
+
+INT_MAX = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("most,win,sinks", [
+    (INT_MAX, 1, INT_MAX), (INT_MAX, 1, INT_MAX - 1), (INT_MAX, 30, INT_MAX), (INT_MAX - 1, 1, INT_MAX), (INT_MAX, 1, 1 << 30),
+    (INT_MAX, 0, INT_MAX), (INT_MAX, 1 << 30, 0)])
+def test_largest_lengths_and_sinks(most, win, sinks):
+    """The tiles of a length near 2^31 are counted without a wrap: about all of them are seen here, so that the call
+    is split as one of 2^30 keys that are all seen is, and needs as large a workspace."""
+    need = pq.lib().pq_paged_decode_workspace_bytes
+    assert need(1, 32, 8, 64, 1 << 30, 0, 0) > 0
+    assert need(1, 32, 8, 64, most, win, sinks) == need(1, 32, 8, 64, 1 << 30, 0, 0)
