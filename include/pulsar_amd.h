@@ -517,15 +517,17 @@ int pq_attn_layer_decode(const uint16_t *qkvg, const float *q_norm, const float 
  *
  * Sequence b holds n = kv_len[b] positions, of which the last c are this
  * call's rows: rows q_start[b] .. q_start[b+1]-1 of its inputs and outputs (c
- * = their count; q_start ascends), or row b alone where q_start is NULL (then
- * a call has nseq rows). Row i of the c is position n - c + i. Position j is
- * slot j % page of page table[b * table_stride + j / page].
+ * = their count), or row b alone where q_start is NULL (then a call has nseq
+ * rows). Row i of the c is position n - c + i. Position j is slot j % page of
+ * page table[b * table_stride + j / page].
  *
  * The lengths and the pages are read on the device, so a captured call replays
  * for other ones. What they hold is checked there, not refused: a page outside
  * [0, npages), and a position past the row's table_pages, holds no key (nothing is
  * read or written for it); kv_len <= 0 is a sequence without keys (a padded
- * batch); rows outside [q_start[0], q_start[nseq]) are left as they were. Pages
+ * batch); of a sequence's rows those that the call has, [0, T), are taken (c
+ * counts all of them); where a start is above the next one, that sequence and
+ * those behind it have no rows; rows of no sequence are left as they were. Pages
  * may be shared between sequences that only read them. */
 typedef struct pq_paged_kv {
   uint16_t *k, *v;         /* pools [npages][page][nkv][hd], fp16 or bf16, 16-byte aligned */

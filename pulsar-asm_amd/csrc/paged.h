@@ -1,5 +1,6 @@
 // paged.h -- what the paged-cache kernels share: the device view of a
-// pq_paged_kv, the row -> (sequence, position) map and the visibility rule.
+// pq_paged_kv, the row -> (sequence, position) map, a position's place in the pools
+// and the output step.
 #pragma once
 #include "pq_device.h"
 #include "pq_host.h"
@@ -24,29 +25,32 @@ int paged_attn_check(const char *who, const uint16_t *q, int q_stride, const pq_
                      int gate_stride, const uint16_t *out, int out_stride, const int8_t *qx, const float *dx, int nh,
                      int win, int sinks, int max_kv, PagedView *v);
 
-// The sequence that row belongs to (the wave's lanes scan q_start together), or
-// -1; first / count: its rows. row must be uniform over the wave.
-__device__ __forceinline__ int paged_seq_of_row(const PagedView &kv, int row, int &first, int &count) {
+// Of 64 lanes' "the start of my sequence is at most the next one's": those before the first that is not.
+__device__ __forceinline__ uint64_t paged_ascending(uint64_t up) { return up & ~(up + 1); }
+
+// The sequence that row of the call belongs to (the wave's lanes scan q_start
+// together), or -1; left: the rows from this one to the sequence's end, so that its
+// position is kv_len - left. A start above the next one ends the sequences: that
+// sequence and those behind it have no rows. row must be uniform over the wave.
+__device__ __forceinline__ int paged_seq_of_row(const PagedView &kv, int row, int &left) {
   if (kv.q_start == nullptr) {
-    first = row;
-    count = 1;
+    left = 1;
     return row < kv.nseq ? row : -1;
   }
   const int lane = threadIdx.x & 63;
-  int b = 0;
-  for (int i = 0; i < kv.nseq; i += 64)
-    b += __popcll(__ballot(i + lane < kv.nseq && kv.q_start[i + lane < kv.nseq ? i + lane + 1 : 0] <= row));
-  if (b >= kv.nseq) return -1;
-  first = kv.q_start[b];
-  const int end = kv.q_start[b + 1];
-  count = end - first;
-  return row >= first && row < end ? b : -1;
-}
-
-// kv_len[b], a length below any call's rows standing for none (so that a row's position does not wrap)
-__device__ __forceinline__ int paged_len(const PagedView &kv, int b) {
-  const int n = kv.kv_len[b];
-  return n < -(1 << 24) ? -(1 << 24) : n;
+  for (int i = 0; i < kv.nseq; i += 64) {
+    const int j = i + lane, jc = j < kv.nseq ? j : kv.nseq - 1;
+    const int first = kv.q_start[jc], next = kv.q_start[jc + 1];
+    const uint64_t up = __ballot(j < kv.nseq && first <= next);
+    const uint64_t hit = __ballot(first <= row && row < next) & paged_ascending(up);
+    if (hit != 0) {
+      const int l = __builtin_ctzll(hit);
+      left = __builtin_amdgcn_readlane(next, l) - row;
+      return i + l;
+    }
+    if (up != ~0ull) break;
+  }
+  return -1;
 }
 
 // Element offset of position j's row of kv heads in the pools, or -1 when it

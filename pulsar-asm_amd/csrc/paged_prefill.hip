@@ -113,26 +113,32 @@ __global__ __launch_bounds__(64 * NW, HD == 64 && NW == 4 ? 3 : 2) void paged_pr
   const int g = blockIdx.x % kv.nkv, slot = slots - 1 - blockIdx.x / kv.nkv;
   const int G = A.G, kvd = kv.nkv * HD;
   // the sequence of the slot, its rows and its length: lane j reads sequence i + j's, the last one that starts at the
-  // slot or before is taken
+  // slot or before is taken, of those up to a start that does not ascend (as paged_seq_of_row has them)
   int b = -1, q0 = 0, q1 = 0, len = 0;
   for (int i = 0; i < kv.nseq; i += 64) {
     const int j = i + lane, jc = j < kv.nseq ? j : kv.nseq - 1;
     const int first = kv.q_start != nullptr ? kv.q_start[jc] : jc, next = kv.q_start != nullptr ? kv.q_start[jc + 1] : jc + 1;
-    const int n = paged_len(kv, jc);
-    const int at = j < kv.nseq ? (first > 0 ? (int)((long long)first * G / BM) : 0) + j : 0x7fffffff;
-    const int before = __popcll(__ballot(at <= slot));
+    const int n = kv.kv_len[jc];
+    const int at = (first > 0 ? (int)((long long)first * G / BM) : 0) + j;
+    const uint64_t up = __ballot(j < kv.nseq && first <= next);
+    const int before = __popcll(__ballot(at <= slot) & paged_ascending(up));
     if (before == 0) break;
     b = i + before - 1;
     q0 = __builtin_amdgcn_readlane(first, before - 1);
     q1 = __builtin_amdgcn_readlane(next, before - 1);
     len = __builtin_amdgcn_readlane(n, before - 1);
+    if (up != ~0ull) break;
   }
   if (b < 0) return;
-  if (q0 < 0 || q1 > A.T || q1 <= q0) return;
+  // its rows within the call's, and the position of the first: row i of them is at p0 + i. Below -2^24 none of 2^23 rows
+  // has one
+  if (q0 < 0) q0 = 0;
+  const int left = q1 - q0;
+  if (q1 > A.T) q1 = A.T;
+  if (q1 <= q0) return;
   const int rows = (q1 - q0) * G, r0 = (slot - ((int)((long long)q0 * G / BM) + b)) * BM;
-  if (r0 < 0 || r0 >= rows) return;   // below 0: q_start does not ascend
-  // positions: row i of the sequence is at p0 + i
-  const int p0 = len - (q1 - q0);
+  if (r0 >= rows) return;
+  const int p0 = (long long)len - left > -(1 << 24) ? len - left : -(1 << 24);
   const int rlast = r0 + BM < rows ? r0 + BM - 1 : rows - 1;
   const int pmin = p0 + r0 / G, pmax = p0 + rlast / G;
   const int limit = pmax + 1 < kv.cap ? pmax + 1 : kv.cap;                 // keys from here on are no row's
@@ -499,9 +505,16 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillArgs A, 
   const int d0 = 4 * (int)(e % TH);
   const long long rh = e / TH;
   const int row = (int)(rh / A.nh), head = (int)(rh % A.nh);
-  if (row >= A.T) return;
-  const int q0 = kv.q_start != nullptr ? kv.q_start[0] : 0, q1 = kv.q_start != nullptr ? kv.q_start[kv.nseq] : kv.nseq;
-  if (row < q0 || row >= q1) return;
+  // whether a sequence has the row, for each of the wave's rows (two or four heads): others have no parts
+  bool mine = false;
+  for (uint64_t todo = __ballot(row < A.T); todo != 0;) {
+    const int r = __builtin_amdgcn_readlane(row, __builtin_ctzll(todo));
+    int left;
+    const bool has = paged_seq_of_row(kv, r, left) >= 0;
+    mine = row == r ? has : mine;
+    todo &= ~__ballot(row == r);
+  }
+  if (!mine) return;
   const size_t p0 = (size_t)rh * A.nsplit;
   const float2 *ml = reinterpret_cast<const float2 *>(A.pml) + p0;
   float M = -__builtin_inff(), L = 0.0f, a[4] = {0, 0, 0, 0};

@@ -79,11 +79,12 @@ __global__ __launch_bounds__(256) void paged_prep_kernel(const uint16_t *qkv, in
   const long long id = (long long)blockIdx.x * 4 + w;
   const int row = (int)(id / parts), h0 = (int)(id % parts) * U * turns;
   if (row >= T) return;
-  int first, count;
-  const int b = paged_seq_of_row(kv, row, first, count);
+  int left;
+  const int b = paged_seq_of_row(kv, row, left);
   if (b < 0) return;
-  const int pos = paged_len(kv, b) - count + (row - first);
-  if (pos < 0 || pos >= rope_rows) return;
+  const int len = kv.kv_len[b];
+  if (len < left || len - left >= rope_rows) return;
+  const int pos = len - left;
   const long long at = paged_row(kv, b, pos, kvd);
   const int half = rot / 2;
   // the cosines and sines of this lane's pairs; 1 and 0 past the rotated dims

@@ -557,3 +557,51 @@ def test_lengths_and_sinks_near_the_largest_int(pq, dev, cache, nh, nkv, hd):
                         o, size, slack = pc.attend64(bt.rows[b:b + 1, :nh * hd].view(1, nh, hd), p, bt.keys[b], bt.vals[b],
                                                      0.1, win, sinks)
                         pc.check(got[b:b + 1], o, pc.tolerance(o, size, slack, bt.n[b], cache))
+
+
+@pytest.mark.parametrize("cache,nh,nkv,hd", [(F16, 8, 2, 64), (BF16, 3, 1, 128)])
+def test_rows_that_belong_to_a_sequence(pq, dev, cache, nh, nkv, hd):
+    """Row r is sequence b's where q_start[b] <= r < q_start[b + 1], whether the starts run past the call's rows at
+    either end or stop to ascend (then b's before that): the cache write and the attention, in one piece and in
+    splits, agree on them, give the rows of a sequence their output and leave the others as they were."""
+    T, lens = 90, [2040, 530, 40]
+    bt = pc.Batch(dev, [40, 30, 20], [a - b for a, b in zip(lens, (40, 30, 20))], nh, nkv, hd, 16, cache, seed=36)
+    one, cs = torch.ones(hd, device=dev), torch.ones((2100, 16, 2), device=dev)
+    L = pq.lib()
+    sizes = {hint: L.pq_paged_prefill_workspace_bytes(3, T, nh, nkv, hd, hint, 0, 0) for hint in (1, 2040)}
+    assert sizes[1] == 0 and sizes[2040] > 0             # in one piece, in splits
+    for starts in ([0, 40, 70, 90], [0, 40, 70, 95], [0, 40, 70, 2 ** 31 - 1], [-5, 40, 70, 200], [-2 ** 31, 40, 90, 90],
+                   [0, 40, 10, 20], [0, 40, 0, 0], [3, 40, 40, 90], [90, 60, 30, 0], [0, 1 << 30, 5, 90], [95, 96, 97, 98],
+                   [0, 0, 0, 89]):
+        print(starts, flush=True)
+        bt.q_start.copy_(torch.tensor(starts))
+        mine = torch.zeros(T, dtype=torch.bool, device=dev)
+        there = torch.zeros(T, dtype=torch.bool, device=dev)
+        want = torch.zeros((T, nh, hd), dtype=torch.float64, device=dev)
+        tol = torch.zeros_like(want)
+        for b in range(3):
+            if starts[b] > starts[b + 1]:
+                break
+            r = torch.arange(max(starts[b], 0), max(min(starts[b + 1], T), max(starts[b], 0)), device=dev)
+            p = lens[b] - starts[b + 1] + r
+            if not len(r):
+                continue
+            rows = bt.rows[r]
+            o, size, slack = pc.attend64(rows[:, :nh * hd].view(-1, nh, hd), p, bt.keys[b], bt.vals[b], 0.1, 0, 0,
+                                         rows[:, bt.width - nh:bt.width])
+            want[r], tol[r], mine[r] = o, pc.tolerance(o, size, slack, lens[b], cache), True
+            there[r] = p >= 0
+        for hint in (1, 2040):
+            out = torch.full((T + 8, nh * hd), 5.0, dtype=BF16, device=dev)
+            ws = torch.full((max(sizes[hint], 16) // 4,), 1e30, device=dev)
+            pq.paged_attn_prefill(bt.view(pq), bt.rows, nh, 0.1, gate=bt.gate, max_kv=hint, out=out[4:-4], ws=ws)
+            got = out[4:-4]
+            assert (out[:4] == 5).all() and (out[-4:] == 5).all()
+            assert (got[~mine] == 5).all(), (hint, "a row of no sequence was written")
+            pc.check(got[mine], want[mine], tol[mine])
+        # the cache write takes the same rows, those whose position there is
+        k, v = bt.k_all.clone(), bt.v_all.clone()
+        q = torch.full((T, nh * hd), 5.0, dtype=BF16, device=dev)
+        pq.paged_qk_prep(bt.view(pq), bt.rows, one, one, cs, nh, 32, out=q)
+        assert torch.equal((q != 5).any(1), there)
+        bt.k_all.copy_(k), bt.v_all.copy_(v)
