@@ -212,7 +212,6 @@ __global__ __launch_bounds__(64 * NW, HD == 64 && NW == 4 ? 3 : 2) void paged_pr
   // scaled by the power of two that brings the row's largest value into [1, 2): exact but for what lies 2^-25 below it
   v4u qf[S];
   float sc = fabsf(A.scale) * 1.44269504088896341f;
-  if (sc == 0.0f) sc = 0x1p-126f;   // a scale of 0: weights of 1, and a hidden score's product still -infinity
   {
     const uint16_t *qr = A.q + (size_t)row * A.q_stride + (size_t)head * HD + 8 * h;
     const uint32_t flip = A.scale < 0.0f ? 0x80008000u : 0u;
@@ -244,6 +243,9 @@ __global__ __launch_bounds__(64 * NW, HD == 64 && NW == 4 ? 3 : 2) void paged_pr
           qf[s][i] = pack2<false>(__builtin_amdgcn_ldexpf(__uint_as_float(qf[s][i] << 16), -e),
                                   __builtin_amdgcn_ldexpf(__uint_as_float(qf[s][i] & 0xffff0000u), -e));
     }
+    // 0 as the scale or what is left of it: the least number, so that a hidden score's product is still -infinity and
+    // any finite one's below 2^-21, the weights 1
+    if (sc == 0.0f) sc = 0x1p-149f;
   }
 
   // LDS addresses: K's row swap(m) of a 32-key half, chunk 2 s + h; V's key and dims of the transposing read

@@ -605,3 +605,31 @@ def test_rows_that_belong_to_a_sequence(pq, dev, cache, nh, nkv, hd):
         pq.paged_qk_prep(bt.view(pq), bt.rows, one, one, cs, nh, 32, out=q)
         assert torch.equal((q != 5).any(1), there)
         bt.k_all.copy_(k), bt.v_all.copy_(v)
+
+
+@pytest.mark.parametrize("cache,hd", [(F16, 64), (F16, 128), (BF16, 64), (BF16, 128)])
+def test_scales_beside_small_and_large_queries(pq, dev, cache, hd):
+    """A scale of 0, or so small that it vanishes beside the queries', leaves every visible key one weight, whatever
+    the queries are: the values' mean, beside keys that are hidden."""
+    nh, nkv = 8, 2
+    bt = pc.Batch(dev, [70, 1], [30, 200], nh, nkv, hd, 16, cache, seed=37)
+    rows = bt.rows.clone()
+    big = 2.0 ** 60 if cache == BF16 else 2.0 ** 100
+    keys = [k.clone() for k in bt.keys]
+    for scale, size, kscale in ((0.0, 1.0, 1.0), (0.0, 2.0 ** -30, 1.0), (0.0, 2.0 ** -132, 1.0), (2.0 ** -20, 2.0 ** -132, 1.0),
+                                (2.0 ** -140, 2.0 ** -10, 1.0), (0.0, big, 2.0 ** 60 if cache == BF16 else 1.0),
+                                (-(2.0 ** -149), 2.0 ** -20, 1.0), (0.125, 0.0, 1.0)):
+        print(scale, size, flush=True)
+        bt.rows.copy_(rows)
+        bt.rows[:, :nh * hd] *= size
+        bt.keys = [k * kscale for k in keys]
+        bt.store()
+        for win, sinks in ((0, 0), (40, 2)):
+            want, tol = pc.want(bt, 0.0, win, sinks)
+            assert (tol < 0.1).all() or size == big
+            one = pq.PagedKV(bt.k, bt.v, bt.table[1:], bt.kv_len[1:])
+            tol = torch.minimum(tol, torch.full_like(tol, 0.1))
+            for hint in (1, 4000):
+                kw = dict(win=win, sinks=sinks, max_kv=hint)
+                pc.check(pq.paged_attn_prefill(bt.view(pq), bt.rows, nh, scale, gate=bt.gate, **kw), want, tol)
+                pc.check(pq.paged_attn_decode(one, bt.rows[70:], nh, scale, gate=bt.gate[70:], **kw), want[70:], tol[70:])
