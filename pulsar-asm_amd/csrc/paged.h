@@ -62,7 +62,14 @@ __device__ __forceinline__ long long paged_row(const PagedView &kv, int b, int j
   return id * kv.page_stride + (long long)(j & ((1 << kv.lg_page) - 1)) * kvd;
 }
 
-// fp16 or bf16 cache element -> f32 and back
+// A finite scale's multiplier of the scores, cut to the finite ones where the queries' exponent takes it past them: a
+// score of 0 stays 0.
+__device__ __forceinline__ float paged_finite(float sc, float scale) {
+  constexpr float most = 0x1.fffffep127f;
+  return fabsf(scale) <= most ? fminf(fmaxf(sc, -most), most) : sc;
+}
+
+// fp16 or bf16 cache element -> f32
 template <bool BF>
 __device__ __forceinline__ float kv2f(uint16_t v) {
   if constexpr (BF) return bf2f(v);

@@ -256,6 +256,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_split_kernel(
           qf[s][i] = f2h2(__builtin_amdgcn_ldexpf(__uint_as_float(qf[s][i] << 16), -e),
                           __builtin_amdgcn_ldexpf(__uint_as_float(qf[s][i] & 0xffff0000u), -e));
     }
+    sc = paged_finite(sc, scale);
     // fp16 weights are held as 2^14 of theirs: what is lost below fp16's range is then 2^-39 of the largest
     constexpr float kLift = BF ? 0.0f : 14.0f;
     float m = -__builtin_inff(), l = 0.0f;

@@ -246,6 +246,7 @@ __global__ __launch_bounds__(64 * NW, HD == 64 && NW == 4 ? 3 : 2) void paged_pr
     // 0 as the scale or what is left of it: the least number, so that a hidden score's product is still -infinity and
     // any finite one's below 2^-21, the weights 1
     if (sc == 0.0f) sc = 0x1p-149f;
+    sc = paged_finite(sc, A.scale);
   }
 
   // LDS addresses: K's row swap(m) of a 32-key half, chunk 2 s + h; V's key and dims of the transposing read

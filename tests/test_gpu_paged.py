@@ -633,3 +633,23 @@ def test_scales_beside_small_and_large_queries(pq, dev, cache, hd):
                 kw = dict(win=win, sinks=sinks, max_kv=hint)
                 pc.check(pq.paged_attn_prefill(bt.view(pq), bt.rows, nh, scale, gate=bt.gate, **kw), want, tol)
                 pc.check(pq.paged_attn_decode(one, bt.rows[70:], nh, scale, gate=bt.gate[70:], **kw), want[70:], tol[70:])
+
+
+@pytest.mark.parametrize("cache,hd", [(F16, 64), (F16, 128), (BF16, 64), (BF16, 128)])
+def test_scales_that_outgrow_fp32(pq, dev, cache, hd):
+    """A scale whose product with the queries' size is past fp32 leaves a score of 0 what it is: keys of zero have one
+    weight each, also where a whole tile is seen and where a part of one is."""
+    nh, nkv = 8, 2
+    bt = pc.Batch(dev, [70, 1], [130, 300], nh, nkv, hd, 16, cache, seed=38)
+    bt.keys = [k * 0.0 for k in bt.keys]
+    bt.store()
+    rows = torch.sign(bt.rows[:, :nh * hd].clone())
+    one = pq.PagedKV(bt.k, bt.v, bt.table[1:], bt.kv_len[1:])
+    for scale, size in ((2.0, 2.0 ** 127), (-4.0, 2.0 ** 127), (2.0 ** 120, 2.0 ** 20), (3e38, 1.0)):
+        bt.rows[:, :nh * hd] = rows * size
+        for win, sinks in ((0, 0), (40, 2)):
+            want, tol = pc.want(bt, 0.0, win, sinks)
+            for hint in (1, 4000):
+                kw = dict(win=win, sinks=sinks, max_kv=hint)
+                pc.check(pq.paged_attn_prefill(bt.view(pq), bt.rows, nh, scale, gate=bt.gate, **kw), want, tol)
+                pc.check(pq.paged_attn_decode(one, bt.rows[70:], nh, scale, gate=bt.gate[70:], **kw), want[70:], tol[70:])
