@@ -480,8 +480,8 @@ class PagedKV:
         if any(t.dtype != torch.int32 for t in ints):
             raise ValueError("table, kv_len and q_start must be int32")
         if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1 or table.stride(1) != 1 \
-                or table.stride(0) < table.shape[1]:
-            raise ValueError("table must be [nseq][pages] with unit column stride")
+                or table.stride(0) < table.shape[1] or max(table.stride(0), table.shape[0]) > _INT_MAX:
+            raise ValueError("table must be [nseq][pages] with unit column stride, its sizes and row stride below 2^31")
         nseq = table.shape[0]
         if tuple(kv_len.shape) != (nseq,) or not kv_len.is_contiguous():
             raise ValueError("kv_len must be a contiguous [nseq] tensor")
@@ -509,6 +509,8 @@ def _paged_rows(kv, what, t, width):
     shape, stride = t.shape, t.stride()
     if len(shape) != 2 or shape[1] < width or stride[1] != 1 or t.dtype not in _RAW16 or t.device != kv.device:
         raise ValueError(f"{what} must be bf16 rows of at least {width} on the cache's device, unit column stride")
+    if stride[0] > _INT_MAX:
+        raise ValueError(f"{what}'s row stride must be below 2^31")
     return t.data_ptr(), stride[0], shape[0]
 
 
@@ -527,6 +529,8 @@ def paged_qk_prep(kv, qkv, q_norm, k_norm, rope_cs, nh, rot, eps=1e-5, out=None)
     (pq_paged_qk_prep): qkv rows [q | k | v | ...], rope_cs [positions][rot/2][2]
     fp32. Returns q [T][nh * hd] (bf16; out may be qkv itself: in place)."""
     hd, nkv = kv.hd, kv.nkv
+    if nh < 1:
+        raise ValueError("nh must be at least 1")
     x, xs, T = _paged_rows(kv, "qkv", qkv, (nh + 2 * nkv) * hd)
     if any(t.dtype != torch.float32 or not t.is_contiguous() or t.device != kv.device for t in (q_norm, k_norm, rope_cs)):
         raise ValueError("the norm weights and the RoPE table must be contiguous fp32 on the cache's device")
@@ -538,11 +542,13 @@ def paged_qk_prep(kv, qkv, q_norm, k_norm, rope_cs, nh, rot, eps=1e-5, out=None)
     if Ty != T:
         raise ValueError("out must have a row for each of qkv's")
     check(lib().pq_paged_qk_prep(x, xs, y, ys, q_norm.data_ptr(), k_norm.data_ptr(), rope_cs.data_ptr(),
-                                 rope_cs.shape[0], kv.ref, nh, rot, T, eps, _paged_stream(kv)), "pq_paged_qk_prep")
+                                 min(rope_cs.shape[0], _INT_MAX), kv.ref, nh, rot, T, eps, _paged_stream(kv)), "pq_paged_qk_prep")
     return out
 
 
 def _paged_attn(kv, q, nh, scale, gate, win, sinks, max_kv, out, qx, dx, ws, prefill):
+    if nh < 1:
+        raise ValueError("nh must be at least 1")
     n = nh * kv.hd
     qp, qs, T = _paged_rows(kv, "q", q, n)
     if not prefill and T != kv.nseq:
@@ -565,7 +571,7 @@ def _paged_attn(kv, q, nh, scale, gate, win, sinks, max_kv, out, qx, dx, ws, pre
         raise ValueError("qx must be int8 [T][nh * hd], dx fp32 [T][nh * hd / 32], contiguous on the cache's device")
     if max_kv is None:
         max_kv = kv.capacity
-    if not (0 <= win <= 1 << 30 and 0 <= sinks <= _INT_MAX and 0 < max_kv <= _INT_MAX and nh <= _INT_MAX):
+    if not (0 <= win <= 1 << 30 and 0 <= sinks <= _INT_MAX and 0 < max_kv <= _INT_MAX):
         raise ValueError("win must be 0 .. 2^30, sinks and max_kv must fit an int, max_kv above 0")
     L = lib()
     if ws is None:

@@ -137,3 +137,29 @@ def test_largest_lengths_and_sinks(most, win, sinks):
     need = pq.lib().pq_paged_decode_workspace_bytes
     assert need(1, 32, 8, 64, 1 << 30, 0, 0) > 0
     assert need(1, 32, 8, 64, most, win, sinks) == need(1, 32, 8, 64, 1 << 30, 0, 0)
+
+
+def test_sizes_past_an_int():
+    """The library's sizes are ints: a stride or a count that does not fit one is refused, not cut to its low 32 bits
+    (the storage is never touched)."""
+    k, v, t, n = _tensors()
+    start = torch.zeros(3, dtype=torch.int32)
+    kv = pq.PagedKV(k, v, t, n, start)
+    rows = torch.zeros((2, 3104), dtype=torch.bfloat16)
+    far = torch.empty_strided((2, 3104), ((1 << 32) + 3104, 1), dtype=torch.bfloat16)
+    w, cs = torch.ones(64), torch.zeros((40, 16, 2))
+    for kw in (dict(qkv=far), dict(qkv=rows, out=far)):
+        with pytest.raises(ValueError, match="stride"):
+            pq.paged_qk_prep(kv, q_norm=w, k_norm=w, rope_cs=cs, nh=32, rot=32, **kw)
+    for call in (pq.paged_attn_decode, pq.paged_attn_prefill):
+        for kw in (dict(q=far), dict(q=rows, gate=far), dict(q=rows, out=far)):
+            with pytest.raises(ValueError, match="stride"):
+                call(kv, nh=32, scale=0.125, **kw)
+        for nh in (32 - (1 << 32), 0, -8):
+            with pytest.raises(ValueError, match="nh"):
+                call(kv, rows, nh, 0.125)
+    with pytest.raises(ValueError, match="nh"):
+        pq.paged_qk_prep(kv, rows, w, w, cs, 32 - (1 << 32), 32, out=rows)
+    wide = torch.empty_strided((2, 3), ((1 << 32) + 3, 1), dtype=torch.int32)
+    with pytest.raises(ValueError, match="table"):
+        pq.PagedKV(k, v, wide, n, start)
