@@ -473,15 +473,18 @@ class PagedKV:
         if k.dtype not in _DT_OF or v.dtype != k.dtype or k.dim() != 4 or v.shape != k.shape:
             raise ValueError("k and v must be fp16 or bf16 pools [npages][page][nkv][hd] of one shape")
         npages, page, nkv, hd = k.shape
-        for t in (k, v):
-            if t.stride()[1:] != (nkv * hd, hd, 1) or t.stride(0) != k.stride(0):
-                raise ValueError("a pool's pages must be contiguous, and k and v of one page stride")
+        # the stride of a dimension of size 1 says nothing
+        step = [t.stride(0) if npages > 1 else page * nkv * hd for t in (k, v)]
+        if not k[:1].is_contiguous() or not v[:1].is_contiguous() or step[0] != step[1]:
+            raise ValueError("a pool's pages must be contiguous, and k and v of one page stride")
         ints = [table, kv_len] + ([q_start] if q_start is not None else [])
         if any(t.dtype != torch.int32 for t in ints):
             raise ValueError("table, kv_len and q_start must be int32")
-        if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1 or table.stride(1) != 1 \
-                or table.stride(0) < table.shape[1] or max(table.stride(0), table.shape[0]) > _INT_MAX:
-            raise ValueError("table must be [nseq][pages] with unit column stride, its sizes and row stride below 2^31")
+        if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1 or (table.stride(1) != 1 and table.shape[1] > 1):
+            raise ValueError("table must be [nseq][pages] with unit column stride")
+        row = table.stride(0) if table.shape[0] > 1 else max(table.stride(0), table.shape[1])
+        if row < table.shape[1] or max(row, table.shape[0]) > _INT_MAX:
+            raise ValueError("table's rows must lie apart, its sizes and row stride be below 2^31")
         nseq = table.shape[0]
         if tuple(kv_len.shape) != (nseq,) or not kv_len.is_contiguous():
             raise ValueError("kv_len must be a contiguous [nseq] tensor")
@@ -496,9 +499,9 @@ class PagedKV:
         self.device = k.device
         self.index = k.device.index if k.device.type == "cuda" else None
         c = self.c = PagedKVView()
-        c.k, c.v, c.page_stride = k.data_ptr(), v.data_ptr(), k.stride(0)
+        c.k, c.v, c.page_stride = k.data_ptr(), v.data_ptr(), step[0]
         c.npages, c.page, c.nkv, c.hd, c.dtype = npages, page, nkv, hd, _DT_OF[k.dtype]
-        c.table, c.table_stride, c.table_pages = table.data_ptr(), table.stride(0), table.shape[1]
+        c.table, c.table_stride, c.table_pages = table.data_ptr(), row, table.shape[1]
         c.kv_len = kv_len.data_ptr()
         c.q_start, c.nseq = q_start.data_ptr() if q_start is not None else None, nseq
         self.ref = C.byref(c)
@@ -509,9 +512,12 @@ def _paged_rows(kv, what, t, width):
     shape, stride = t.shape, t.stride()
     if len(shape) != 2 or shape[1] < width or stride[1] != 1 or t.dtype not in _RAW16 or t.device != kv.device:
         raise ValueError(f"{what} must be bf16 rows of at least {width} on the cache's device, unit column stride")
-    if stride[0] > _INT_MAX:
+    step = stride[0]
+    if shape[0] == 1 and not shape[1] <= step <= _INT_MAX:
+        step = shape[1]   # the only row's: says nothing
+    if step > _INT_MAX:
         raise ValueError(f"{what}'s row stride must be below 2^31")
-    return t.data_ptr(), stride[0], shape[0]
+    return t.data_ptr(), step, shape[0]
 
 
 def _paged_stream(kv):

@@ -163,3 +163,24 @@ def test_sizes_past_an_int():
     wide = torch.empty_strided((2, 3), ((1 << 32) + 3, 1), dtype=torch.int32)
     with pytest.raises(ValueError, match="table"):
         pq.PagedKV(k, v, wide, n, start)
+
+
+def test_strides_of_dimensions_of_one():
+    """The stride of a dimension of size 1 says nothing: such tensors, which contiguous() would return as they are, are
+    taken."""
+    n, start = torch.zeros(1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    table = torch.zeros((3, 1), dtype=torch.int32).t()                   # [1][3], strides 1, 1
+    pool = torch.zeros((4, 1, 16, 64), dtype=torch.float16).transpose(1, 2)   # one kv head, [4][16][1][64]
+    assert pool.is_contiguous() and table.is_contiguous()
+    kv = pq.PagedKV(pool, pool.clone(), table, n, start)
+    assert kv.c.page_stride == 16 * 64 and kv.c.table_stride == kv.c.table_pages == 3
+    one = torch.zeros((1, 16, 8, 64), dtype=torch.float16)
+    one = one.as_strided(one.shape, (8, 512, 64, 1))                     # a pool of one page
+    assert pq.PagedKV(one, one, table, n).c.page_stride == 16 * 8 * 64
+    row = torch.zeros((64 * 4, 1), dtype=torch.bfloat16).t()             # one row, strides 1, 1
+    assert row.is_contiguous()
+    for call in (pq.paged_attn_decode, pq.paged_attn_prefill):
+        with pytest.raises(ValueError, match="GPU"):                     # all else is in order
+            call(kv, row, 4, 0.125)
+    assert pq.ops._paged_rows(kv, "q", row, 256)[1:] == (256, 1)
+    assert pq.ops._paged_rows(kv, "q", row[:, :192], 128)[1:] == (192, 1)
