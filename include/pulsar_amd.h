@@ -580,7 +580,8 @@ int pq_paged_attn_decode(const uint16_t *q, int q_stride, const pq_paged_kv *kv,
 /* The same for prompt rows: T rows of a ragged batch (kv->q_start), each row
  * at its position p, with the keys of the sequence's earlier rows in the pages
  * (pq_paged_qk_prep of the batch before it). Rows outside the sequences keep
- * what they held. Weights are rounded to the pool's type for the value product. */
+ * what they held. Weights are rounded to the pool's type for the value product
+ * (those of a bf16 pool for their sum as well). */
 size_t pq_paged_prefill_workspace_bytes(int nseq, int T, int nh, int nkv, int hd, int max_kv, int win, int sinks);
 int pq_paged_attn_prefill(const uint16_t *q, int q_stride, const pq_paged_kv *kv, const uint16_t *gate,
                           int gate_stride, uint16_t *out, int out_stride, int8_t *qx, float *dx, int nh, int T,

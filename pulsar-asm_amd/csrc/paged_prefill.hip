@@ -66,6 +66,11 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
+// c plus both bf16 of w: one dot product with (1, 1), within 1.5 * 2^-23 of the sum
+__device__ __forceinline__ float add_bf2(uint32_t w, float c) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pq_bf16x2, w), __builtin_bit_cast(pq_bf16x2, 0x3f803f80u), c, false);
+}
+
 // the largest of three, NaN if one is
 __device__ __forceinline__ float max3(float a, float b, float c) {
   return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
@@ -299,7 +304,8 @@ __global__ __launch_bounds__(64 * NW, HD == 64 && NW == 4 ? 3 : 2) void paged_pr
     mt = max3(mt, s[1][15], mt);
     return max_half_pair(mt) * sc;
   };
-  // the weights and their sum
+  // The weights and their sum. A bf16 pool's weights lose up to 2^-8 of themselves before the value product, so what is
+  // summed is what is left of them: the roundings then weigh the values and do not scale the output.
   auto weights = [&](const v16f(&s)[2], v4u(&p)[4]) {
     const float off = (mx == -__builtin_inff() ? 0.0f : mx) - kLift;
     float ls[4] = {0, 0, 0, 0};
@@ -309,8 +315,10 @@ __global__ __launch_bounds__(64 * NW, HD == 64 && NW == 4 ? 3 : 2) void paged_pr
       for (int i = 0; i < 16; i += 2) {
         const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], sc, -off));
         const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i + 1], sc, -off));
-        ls[(i >> 1) & 3] += x0 + x1;
-        p[2 * u + (i >> 3)][(i & 7) >> 1] = pack2<BF>(x0, x1);
+        if constexpr (!BF) ls[(i >> 1) & 3] += x0 + x1;
+        const uint32_t w = pack2<BF>(x0, x1);
+        p[2 * u + (i >> 3)][(i & 7) >> 1] = w;
+        if constexpr (BF) ls[(i >> 1) & 3] = add_bf2(w, ls[(i >> 1) & 3]);
       }
     l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
   };

@@ -653,3 +653,27 @@ def test_scales_that_outgrow_fp32(pq, dev, cache, hd):
                 kw = dict(win=win, sinks=sinks, max_kv=hint)
                 pc.check(pq.paged_attn_prefill(bt.view(pq), bt.rows, nh, scale, gate=bt.gate, **kw), want, tol)
                 pc.check(pq.paged_attn_decode(one, bt.rows[70:], nh, scale, gate=bt.gate[70:], **kw), want[70:], tol[70:])
+
+
+@pytest.mark.parametrize("cache,nh,nkv,hd", [(F16, 8, 2, 64), (F16, 4, 1, 128), (BF16, 8, 2, 64), (BF16, 4, 1, 128)])
+def test_mean_of_equal_values(pq, dev, cache, nh, nkv, hd):
+    """Where every visible value is one number, so is the output, to the bit: the weights' sum is that of the weights
+    that meet the values, as they are rounded, and fp32 sums of 700 of them are off by far less than half a step."""
+    bt = pc.Batch(dev, [150, 3, 40], [550, 40, 0], nh, nkv, hd, 16, cache, seed=39)
+    g = torch.Generator()
+    g.manual_seed(40)
+    for b in range(3):
+        row = (1 + torch.rand((1, nkv, hd), generator=g)).to(dev).to(BF16).to(cache)
+        bt.vals[b] = row.expand(bt.n[b], nkv, hd).clone()
+    bt.store()
+    for scale in (0.03, 0.125, 1.0):
+        for win, sinks in ((0, 0), (100, 3)):
+            for hint in (1, 700):
+                got = pq.paged_attn_prefill(bt.view(pq), bt.rows, nh, scale, win=win, sinks=sinks, max_kv=hint)
+                for b in range(3):
+                    want = bt.vals[b][0].to(BF16).repeat_interleave(nh // nkv, 0).view(-1)
+                    rows = got[bt.starts[b]:bt.starts[b + 1]]
+                    assert (rows == want).all(), f"{int((rows != want).sum())} of {rows.numel()} at {scale} {win} {hint}"
+                last = torch.tensor([bt.starts[b + 1] - 1 for b in range(3)], device=dev)
+                one = pq.paged_attn_decode(bt.view(pq, False), bt.rows[last], nh, scale, win=win, sinks=sinks, max_kv=hint)
+                assert torch.equal(one, got[last])
