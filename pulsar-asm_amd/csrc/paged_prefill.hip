@@ -105,9 +105,10 @@ struct PrefillArgs {
 
 // Grid (row tiles x kv heads, splits). Slot s of the row tiles: sequence b has the
 // slots from floor(q_start[b] G / BM) + b on, one more than it can need at most.
-// Three waves a SIMD where head_dim 64 leaves the registers for it (8192 queries 408 -> 392 us).
+// Three waves a SIMD for head_dim 64 (8192 queries 408 -> 392 us), two for 128. Of the fp16 forms 7 and 5 registers are
+// spilled for it, outside the inner run.
 template <int HD, bool BF, int NW>
-__global__ __launch_bounds__(64 * NW, HD == 64 && NW == 4 ? 3 : 2) void paged_prefill_kernel(PrefillArgs A, PagedView kv, int slots) {
+__global__ __launch_bounds__(64 * NW, HD == 64 ? 3 : 2) void paged_prefill_kernel(PrefillArgs A, PagedView kv, int slots) {
   constexpr int BM = 32 * NW, S = HD / 16, N = HD / 32, RB = HD * 2;       // rows, score steps, dim tiles, bytes a row
   constexpr int TB = kKeys * RB, RPI = 1024 / RB, LI = TB / 1024 / NW;     // bytes a tile, rows and a wave's loads
   static_assert(LI >= 1, "a wave loads whole pieces");
@@ -632,19 +633,14 @@ extern "C" int pq_paged_attn_prefill(const uint16_t *q, int q_stride, const pq_p
   A.qvec = aligned(q, 16) && q_stride % 8 == 0 ? 1 : 0;
   A.ovec = aligned(out, 8) && out_stride % 4 == 0 ? 1 : 0;
   hipStream_t st = as_stream(stream);
-#define PQ_PRE(HH, BB)                                        \
-  do {                                                        \
-    if (p.nw == 8) prefill_launch<HH, BB, 8>(A, v, p, st);    \
-    else prefill_launch<HH, BB, 4>(A, v, p, st);              \
+#define PQ_PRE(BB)                                             \
+  do {                                                         \
+    if (hd == 64) prefill_launch<64, BB, 4>(A, v, p, st);      \
+    else if (p.nw == 4) prefill_launch<128, BB, 4>(A, v, p, st); \
+    else prefill_launch<128, BB, 8>(A, v, p, st);              \
   } while (0)
-  const bool bf = kv->dtype == PQ_DTYPE_BF16;
-  if (hd == 64) {
-    if (bf) PQ_PRE(64, true);
-    else PQ_PRE(64, false);
-  } else {
-    if (bf) PQ_PRE(128, true);
-    else PQ_PRE(128, false);
-  }
+  if (kv->dtype == PQ_DTYPE_BF16) PQ_PRE(true);
+  else PQ_PRE(false);
 #undef PQ_PRE
   const int rl = check_launch(who);
   if (rl || p.nsplit == 1) return rl;
