@@ -182,10 +182,10 @@ __global__ __launch_bounds__(64 * NW, HD == 64 ? 3 : 2) void paged_prefill_kerne
   // Written as asm so that its completion is waited for where the tile is taken up and not at every read of LDS.
   const uint32_t lds0 = (uint32_t)(size_t)(lds_char *)smem;
   auto dma = [&](const char *src, uint32_t off, uint32_t dst) {   // src uniform
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds0 + dst), "v"(off), "s"(src) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds0 + dst), "v"(off), "s"(src) : "memory", "m0");
   };
   auto dma_each = [&](const char *src, uint32_t dst) {            // src each lane's own
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds0 + dst), "v"(src) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds0 + dst), "v"(src) : "memory", "m0");
   };
   const char *const kbase = reinterpret_cast<const char *>(kv.k + g * HD), *const vbase = reinterpret_cast<const char *>(kv.v + g * HD);
   const long long pstride = kv.page_stride * 2;
