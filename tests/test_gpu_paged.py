@@ -677,3 +677,122 @@ def test_mean_of_equal_values(pq, dev, cache, nh, nkv, hd):
                 last = torch.tensor([bt.starts[b + 1] - 1 for b in range(3)], device=dev)
                 one = pq.paged_attn_decode(bt.view(pq, False), bt.rows[last], nh, scale, win=win, sinks=sinks, max_kv=hint)
                 assert torch.equal(one, got[last])
+
+
+# ------------------------------------------------- the forms that large calls take
+def _rows_of(bt):
+    """Every row's sequence and position."""
+    seq = [b for b in range(bt.B) for _ in range(bt.q[b])]
+    pos = [bt.n[b] - bt.q[b] + i for b in range(bt.B) for i in range(bt.q[b])]
+    return seq, pos
+
+
+@pytest.mark.parametrize("nh,nkv,cache,q,past,win,sinks", [
+    (16, 16, F16, [2500, 1, 777, 601], [0, 1300, 5, 64], 0, 0),
+    (16, 4, BF16, [2101, 0, 1301, 700], [500, 7, 0, 1100], 0, 0),
+    (16, 4, F16, [2101, 3, 1301, 700], [500, 7, 0, 1100], 1024, 5),
+    (16, 16, BF16, [2500, 1, 777, 601], [0, 1300, 5, 64], 1000, 24)])
+def test_prefill_of_256_row_tiles(pq, dev, nh, nkv, cache, q, past, win, sinks):
+    """The kernel of 8 waves: head_dim 128, row tiles of 256 for each kv head that fill 256 CUs, 1024 keys or more
+    and no shorter window. Some rows see infinite and NaN values, some have left them behind."""
+    hd, page = 128, 32
+    bt = pc.Batch(dev, q, past, nh, nkv, hd, page, cache, seed=101, pad=3)
+    assert -(-bt.T * (nh // nkv) // 256) * nkv >= 256 and max(bt.n) >= 1024 and (win == 0 or win + sinks >= 1024)
+    bt.vals[0][1500, 0, 3] = float("inf")
+    bt.vals[0][1777, nkv - 1, 100] = float("nan")
+    bt.vals[2][40, 1, 64] = -float("inf")
+    bt.vals[2][2, 0, 9] = float("inf")
+    bt.keys[3][200, 2] = float("nan")
+    bt.vals[3][200, 2] = float("nan")
+    bt.store()
+    want, tol = pc.want(bt, hd ** -0.5, win, sinks)
+    mine = ~torch.isnan(want).all(-1).all(-1)
+    out = torch.full((bt.T, nh * hd), 5.0, dtype=BF16, device=dev)
+    qx = torch.full((bt.T, nh * hd), 99, dtype=torch.int8, device=dev)
+    dx = torch.full((bt.T, nh * hd // 32), 99.0, device=dev)
+    pq.paged_attn_prefill(bt.view(pq), bt.rows, nh, hd ** -0.5, gate=bt.gate, win=win, sinks=sinks, max_kv=max(bt.n), out=out,
+                          qx=qx, dx=dx)
+    pc.check(out[mine], want[mine], tol[mine])
+    assert mine[:sum(q)].all() and not mine[sum(q):].any()
+    assert (out[sum(q):] == 5).all() and (qx[sum(q):] == 99).all() and (dx[sum(q):] == 99).all()
+    rx, rd = pq.q8_quant(out)
+    fine = torch.isfinite(out).view(bt.T, -1, 32).all(-1) & mine[:, None]
+    assert torch.equal(dx[fine], rd[fine]) and torch.equal(qx.view(bt.T, -1, 32)[fine], rx.view(bt.T, -1, 32)[fine])
+
+
+@pytest.mark.parametrize("nh,nkv,hd,rot,cache,q,past", [
+    (32, 8, 64, 32, F16, [1900, 1, 0, 899], [0, 77, 5, 300]), (32, 8, 64, 64, BF16, [2800], [3]),
+    (16, 4, 128, 64, BF16, [1900, 1, 0, 899], [0, 77, 5, 300]), (16, 4, 128, 128, F16, [2800], [3]),
+    (24, 2, 64, 32, F16, [4200], [0])])
+def test_prep_of_many_rows(pq, dev, nh, nkv, hd, rot, cache, q, past):
+    """More than 8192 turns of 64 / (hd / 16) heads: one wave takes a row's heads, turn after turn (the last one short
+    where the heads do not fill it)."""
+    page = 64
+    turn = 64 // (hd // 16)
+    bt = pc.Batch(dev, q, past, nh, nkv, hd, page, cache, seed=102, pad=2)
+    assert bt.T * -(-(nh + 2 * nkv) // turn) > 8192 and nh + 2 * nkv > turn
+    g = torch.Generator()
+    g.manual_seed(2)
+    limit = max(bt.n)
+    cs = _rope(dev, limit, rot, g)
+    qn, kn = (1 + 0.2 * torch.randn(hd, generator=g)).to(dev), (1 + 0.2 * torch.randn(hd, generator=g)).to(dev)
+    k0, v0 = bt.k_all.clone(), bt.v_all.clone()
+    out = torch.full((bt.T, nh * hd), 7.0, dtype=BF16, device=dev)
+    pq.paged_qk_prep(bt.view(pq), bt.rows, qn, kn, cs, nh, rot, eps=EPS, out=out)
+    seq, pos = _rows_of(bt)
+    pages = torch.tensor([bt.pages[b][p // page] for b, p in zip(seq, pos)], device=dev)
+    slots = torch.tensor([p % page for p in pos], device=dev)
+    k, v = bt.k[pages, slots], bt.v[pages, slots]
+    for b in range(bt.B):
+        qq, kk, vv, qs, ks, p, on = _prep64(bt, bt.rows, qn, kn, cs, rot, b, limit)
+        r = slice(bt.starts[b], bt.starts[b + 1])
+        _near(out[r].view(-1, nh, hd), qq, qs, BF16, "q") if bt.q[b] else None
+        _near(k[r], kk, ks, cache, "k") if bt.q[b] else None
+        _near(v[r], vv, torch.zeros_like(vv), cache, "v") if bt.q[b] else None
+    k0[pages, slots], v0[pages, slots] = k, v
+    assert torch.equal(bt.k_all.view(torch.int16), k0.view(torch.int16))
+    assert torch.equal(bt.v_all.view(torch.int16), v0.view(torch.int16))
+    assert (out[sum(q):] == 7).all()
+
+
+@pytest.mark.parametrize("nh,nkv,hd,cache", [(32, 8, 64, F16), (32, 8, 64, BF16), (16, 4, 128, F16), (16, 4, 128, BF16)])
+def test_decode_past_the_caches(pq, dev, nh, nkv, hd, cache):
+    """A call that is said to read 256 MiB or more of keys and values reads them past the caches."""
+    past = [3000, 1, 700, 40]
+    bt = pc.Batch(dev, [1] * 4, past, nh, nkv, hd, 16, cache, seed=103)
+    hint = 1 << 18
+    assert 4 * nkv * (hint // 32) * 32 * 4 * hd >= 256 << 20
+    for win, sinks in ((0, 0), (1 << 18, 3), (1 << 17, 70)):
+        want, tol = pc.want(bt, 0.1, win, sinks)
+        got = pq.paged_attn_decode(bt.view(pq, False), bt.rows, nh, 0.1, gate=bt.gate, win=win, sinks=sinks, max_kv=hint)
+        pc.check(got, want, tol)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_decode_weights_of_16_bits(pq, dev, hd):
+    """A bf16 pool's weights go into the value product as two bf16, 16 bits of them in all: where the values cancel, the
+    output is what the weights' roundings leave, half a step of the second bf16, 2^-16 of a weight at most."""
+    lens = [2, 3, 5, 9, 33, 64, 65, 200] * 4
+    nh = nkv = 4
+    bt = pc.Batch(dev, [1] * len(lens), [n - 1 for n in lens], nh, nkv, hd, 16, BF16, seed=104)
+    bt.rows[:, :nh * hd] *= 0.25
+    scale = 0.125
+    for b, n in enumerate(lens):
+        q = bt.rows[b, :nh * hd].double().view(nh, hd)
+        s = scale * torch.einsum("hd,nhd->hn", q, bt.keys[b].double())
+        w = torch.softmax(s, 1)                          # [nh][n]
+        v = bt.vals[b].double()
+        top = w.argmax(1)
+        for h in range(nh):                              # the key of the largest weight takes the others' sum back
+            rest = w[h] @ v[:, h] - w[h, top[h]] * v[top[h], h]
+            bt.vals[b][top[h], h] = (-rest / w[h, top[h]]).to(BF16)
+    bt.store()
+    want, tol = torch.zeros((len(lens), nh, hd), dtype=torch.float64, device=dev), None
+    tol = torch.zeros_like(want)
+    for b, n in enumerate(lens):
+        o, size, slack = pc.attend64(bt.rows[b:b + 1, :nh * hd].view(1, nh, hd), torch.tensor([n - 1], device=dev), bt.keys[b],
+                                     bt.vals[b], scale, 0, 0)
+        want[b], tol[b] = o[0], (2.0 ** -8 * o.abs() + size * (2.0 ** -16 + slack + (n / 8 + 80) * 2.0 ** -24))[0]
+        assert (tol[b] < 2.0 ** -12 * size[0]).float().mean() > 0.9       # far below one bf16's 2^-8
+    for hint in (1, 1 << 16):
+        pc.check(pq.paged_attn_decode(bt.view(pq, False), bt.rows, nh, scale, max_kv=hint), want, tol)
