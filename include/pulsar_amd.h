@@ -539,13 +539,14 @@ typedef struct pq_paged_kv {
   int table_stride, table_pages;
   const int32_t *kv_len;   /* device [nseq] */
   const int32_t *q_start;  /* device [nseq + 1], or NULL: row b is sequence b's one new position */
-  int nseq;                /* at most 65535, and 2^23 with nkv; a call has at most 2^23 rows */
+  int nseq;                /* at most 65535, and 2^23 with nkv; a call has at most 2^23 rows, and of a prompt call
+                              T * nh / 128 + nseq * nkv is at most 2^22 */
 } pq_paged_kv;
 
 /* The head norm of q and k, RoPE and the cache write (pq_qk_prep) for the T
  * rows of a batch, in one pass: qkv rows [q (nh hd) | k (nkv hd) | v (nkv hd) |
  * ...] of row_stride elements, bf16; q_out rows of q_stride elements, bf16
- * (q_out may be qkv itself with q_stride = row_stride); k and v to the pages.
+ * (q_out may be qkv itself with q_stride = row_stride, else must not overlap it); k and v to the pages.
  * rope_cs [rope_rows][rot/2][cos, sin] (NULL with rot 0); a row whose position is outside [0,
  * rope_rows) is left out: its q_out and its slot keep what they held. The
  * arithmetic is fp32 from the bf16 inputs to one rounding at the end
@@ -569,7 +570,9 @@ int pq_paged_qk_prep(const uint16_t *qkv, int row_stride, uint16_t *q_out, int q
  * the workspace with it; any length is computed whole). The keys are split over
  * workgroups and joined in a fixed order: the same call gives the same bits.
  * out must not overlap q. Weights are rounded to 16 bits of mantissa (fp16: 11)
- * for the value product, everything else is fp32.
+ * for the value product, everything else is fp32: scores and sums past its range
+ * are infinite, and an infinite value under a weight that rounds to 0 (a score 22
+ * below the largest for an fp16 pool, 87 for bf16) may give NaN.
  * ws (16-byte aligned): pq_paged_decode_workspace_bytes, 0 where one workgroup
  * a kv head does it. */
 size_t pq_paged_decode_workspace_bytes(int nseq, int nh, int nkv, int hd, int max_kv, int win, int sinks);

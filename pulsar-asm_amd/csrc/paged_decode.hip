@@ -566,9 +566,17 @@ __global__ __launch_bounds__(kJoin) void paged_join_kernel(const uint16_t *__res
 // these before the reads past the caches below).
 //
 // K and V are read past the caches (once) where they fill the last-level cache of 256
-// MiB, as nothing of them is left there for the next call: 563 MB 112 -> 102 us, 268 MB
-// 58.4 -> 56.2, 128 sequences of up to 4800 keys of 8 heads of 64 151 -> 139; below that a pool
-// that is read again finds some of it there (32 sequences of 1200, 50 MB, 15.8 / 21.8).
+// MiB: 563 MB 112 -> 102 us, 128 sequences of up to 4800 keys of 8 heads of 64 151 -> 139. Through
+// the caches / past them (us), 16 sequences of 8 heads of 64, one pool read again and
+// again: 64 MiB 24.3 / 26.0, 128 33.2 / 36.6, 192 41.9 / 47.4, 256 52.4 / 57.4, 320 70.7 / 69.0,
+// 512 112 / 101; six such pools in turn, as a model's layers are: 64 27.7 / 27.2, 128 38.9 /
+// 37.2, 192 49.7 / 46.9, 256 60.9 / 56.5, 512 110 / 100. A call does not know which it is; the
+// border keeps a pool that fits its place in the cache. Shorter ones lose more: 32 sequences
+// of 1200, 50 MB, 15.8 / 21.8.
+//
+// by_wg, join by head / by workgroup (us), 32 q and 8 kv heads of 64, 4096 keys: 1 sequence 14.9 /
+// 21.9, 8 22.9 / 27.5, 16 33.2 / 33.4, 32 61 / 56, 64 109 / 98; 16 and 4 of 128: 1 14.5 / 33.5, 16 31.8 / 37.9,
+// 32 55 / 57.6, 64 97 / 96, 128 of 2048 102 / 95.
 struct PagedPlan {
   int HW, grid, share, by_wg;
   bool once;

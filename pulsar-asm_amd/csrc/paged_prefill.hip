@@ -22,14 +22,14 @@
 // (no bank conflicts; V's first swizzle had a third of the LDS cycles in them).
 //
 // What bounds it: the matrix cores and the vector unit by turns. A wave's tile is 32
-// products of 32 cycles (head_dim 128; 16 for 64) and about 200 vector instructions,
-// 32 of them e^x; the two waves of a SIMD are at the same step behind each barrier,
-// so the two add up: 40% of the cycles in products, 41% in vector instructions. Tiles
-// that some row sees in part cost half as much again. Measured: 16384 queries of 16 q and
-// 4 kv heads of 128 1.04 to 1.10 ms (1.0 PFLOP/s; a large library product reaches 1.3),
-// 2048 queries behind 14336 in 8 sequences 1.07 PFLOP/s, 8192 queries of 32 and 8 heads of 64
-// 375 us (730 TFLOP/s), 16384 in a window of 256 with 4 sinks 106 us, 512 behind 32000 in 8
-// splits 155 us, ragged prompts of up to 2048 of 32 and 8 heads of 64 137 to 144 us.
+// products of 32 cycles (head_dim 128; 16 for 64) and 150 to 160 vector instructions (137
+// to 145 with a bf16 pool), 32 of them e^x; the two waves of a SIMD are at the same step behind each
+// barrier, so the two add up: 47% of the cycles in products, 43% in vector instructions.
+// Tiles that some row sees in part cost half as much again. Measured: 16384 queries of 16 q
+// and 4 kv heads of 128 1.07 to 1.10 ms (1.0 PFLOP/s; a large library product reaches 1.3),
+// 2048 queries behind 14336 in 8 sequences 1.01 PFLOP/s, 8192 queries of 32 and 8 heads of 64
+// 344 us (800 TFLOP/s), 16384 in a window of 256 with 4 sinks 99 us, 512 behind 32000 in 8
+// splits 155 to 159 us, ragged prompts of up to 2048 of 32 and 8 heads of 64 137 to 145 us.
 #include <type_traits>
 
 #include "paged.h"
@@ -306,7 +306,9 @@ __global__ __launch_bounds__(64 * NW, HD == 64 ? 3 : 2) void paged_prefill_kerne
     return max_half_pair(mt) * sc;
   };
   // The weights and their sum. A bf16 pool's weights lose up to 2^-8 of themselves before the value product, so what is
-  // summed is what is left of them: the roundings then weigh the values and do not scale the output.
+  // summed is what is left of them: the roundings then weigh the values and do not scale the output. (A weight as two
+  // bf16, as in the decode kernel, takes half as many products again: 16384 queries 1067 -> 1448 us, 512 behind 32000
+  // 155 -> 203, for an error of 0.0017 of the outputs' norm where it is 0.0019 to 0.0022; the output's rounding is 0.0017.)
   auto weights = [&](const v16f(&s)[2], v4u(&p)[4]) {
     const float off = (mx == -__builtin_inff() ? 0.0f : mx) - kLift;
     float ls[4] = {0, 0, 0, 0};
@@ -568,10 +570,11 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillArgs A, 
 // fill the chip and see 1024 keys or more (head_dim 128: K and V are then read half as often), else
 // of 128; and splits until one workgroup of 256 rows, or two of 128, a CU have
 // work, each of at least 2 tiles of keys. Measured, 256 / 128 rows (us): 16384 queries of 16 q
-// and 4 kv heads of 128 1082 / 1124, 16 sequences of 4096 1293 / 1353, 32 of 2048 786 / 801,
-// 16384 in a window of 256 127 / 107; head_dim 64, 32 and 8 heads, 8192 queries 448 / 424;
-// 203 queries behind 300 unsplit 26 / 22, in 3 splits of 128 rows 18.6; 512 behind 32000
-// unsplit 838 / 699, in 8 splits of 128 rows 158.
+// and 4 kv heads of 128 1070 / 1133 (fp16 1124 / 1180), 16 sequences of 4096 1251 / 1270, 32 of
+// 2048 727 / 729, 2048 behind 14336 in 8 sequences 2033 / 2121, 16384 in a window of 256
+// 112 / 94; head_dim 64, 32 and 8 heads, 8192 queries 448 / 424 (when it had both); 203 queries
+// behind 300 unsplit 25.4 / 21.3, in 3 splits of 128 rows 17.7; 512 behind 32000 unsplit
+// 856 / 725, in 8 splits of 128 rows 182. Row tiles are counted as if sequences shared them.
 struct PrefillPlan {
   int nw, slots, nsplit;
 };

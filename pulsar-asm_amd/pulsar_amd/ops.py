@@ -608,7 +608,8 @@ def paged_attn_decode(kv, q, nh, scale, gate=None, win=0, sinks=0, max_kv=None, 
     """Attention of one new token a sequence over its pages
     (pq_paged_attn_decode): q rows [nseq][nh * hd ...] bf16, gate rows [nseq][nh].
     win > 0: a sliding window whose first `sinks` tokens stay visible. max_kv:
-    about the largest length (the table's capacity if not given). Returns out
+    about the largest length; the table's capacity if not given, which splits
+    the work, and sizes the workspace, as full tables need it. Returns out
     (bf16 [nseq][nh * hd]); qx / dx receive its Q8_0 form."""
     return _paged_attn(kv, q, nh, scale, gate, win, sinks, max_kv, out, qx, dx, ws, False)
 
